@@ -422,6 +422,80 @@ TP_API int tp_radam_step_multi(const int64_t* params, const int64_t* grads, cons
                                const int64_t* exp_avg_sqs, int n, float lr, float beta1, float beta2, float eps,
                                float weight_decay, float step_size, float beta1_pow_t, float beta2_pow_t,
                                int64_t step);
+/* New: the global norm of many gradients, and clipping by it.  N = (sum
+ * |g|^norm_type)^(1/norm_type) over every value of every tensor, norm_type 1, 2
+ * or inf (summed in f64), coef = min(1, max_norm / (N + 1e-6)); every gradient
+ * is multiplied by coef in place (left alone when coef is 1).  *norm is a new
+ * tensor [2]: N and coef, left in HBM.  A NaN gradient makes both NaN, an
+ * infinite one makes N infinite and coef 0 (NaN if max_norm is infinite too).
+ * max_norm must not be negative; the same gradient listed twice is refused.
+ * No tensors: N = 0. */
+TP_API int tp_clip_grad_norm_multi(const int64_t* grads, int n, float norm_type, float max_norm, tp_handle* norm);
+/* New: the 2-norm of the group's gradients and the AdamW (kind 0) or Adam (1)
+ * step that reads each gradient times coef: the same parameters and moments,
+ * bit for bit, as tp_clip_grad_norm_multi followed by the step, with the
+ * gradients left as they were. */
+TP_API int tp_adam_clip_step_multi(int kind, const int64_t* params, const int64_t* grads, const int64_t* exp_avgs,
+                                   const int64_t* exp_avg_sqs, int n, float lr, float beta1, float beta2, float eps,
+                                   float weight_decay, float step_size, float inv_sqrt_bc2, float max_norm,
+                                   tp_handle* norm);
+
+/* ---- token operators (new: no counterpart on the reference's hot path) -------- */
+/* Token ids are read on the device: float32 storage (truncated toward zero) or
+ * the int32 storage of index outputs, so an argmax or the alternatives below
+ * feed the next lookup without a readback.  Vocabularies go up to 2^24, the
+ * whole numbers float32 holds.  An id outside [0, vocab) reads nothing: its
+ * outputs are NaN (tp_synchronize reports no error), and it adds to no
+ * gradient; where a negative id has a meaning the entry says so. */
+/* Per row of logits [..., vocab] with the ids [...]: logp [...] = log softmax at
+ * the id (0 for a negative id: an ignored row), entropy [...] of the row's
+ * softmax, stats [..., 2] = (max, log of the sum of exp(x - max)) for the
+ * backward pass, and the topk (0..32, <= vocab) most likely tokens, ties to the
+ * lower id: top_ids [..., topk] (int32 storage) and their top_logp [..., topk].
+ * A logit of -inf is a masked token: probability 0, never an alternative
+ * (missing ones: id -1, logp -inf).  A row of -inf only: logp -inf, entropy 0,
+ * stats -inf.  A row with NaN or +inf: NaN, alternatives -1.  An output the
+ * caller passes no handle for is dropped. */
+TP_API int tp_token_logprobs(int64_t logits, int64_t ids, int topk, tp_handle* logp, tp_handle* entropy,
+                             tp_handle* stats, tp_handle* top_ids, tp_handle* top_logp);
+/* gradient of (logp, entropy) with respect to the logits, from the forward's
+ * stats and entropy; dlogp or dentropy may be 0 (no gradient).  With p the
+ * row's softmax: dlogp * ([i = id] - p_i) - dentropy * p_i (log p_i + entropy).
+ * Rows whose upstream gradients are both 0 (or ignored) get zeros whatever
+ * their logits hold, as do rows of -inf only; rows with NaN or +inf get NaN. */
+TP_API int tp_token_logprobs_backward(int64_t dlogp, int64_t dentropy, int64_t logits, int64_t ids, int64_t stats,
+                                      int64_t entropy, tp_handle* out);
+/* out [..., dim] = scale * table[id], table [vocab, dim] */
+TP_API int tp_token_embedding(int64_t table, int64_t ids, float scale, tp_handle* out);
+/* the table's gradient: row v = scale * the sum of grad_out [..., dim] over the
+ * positions whose id is v, in an order fixed by the positions (equal inputs,
+ * equal bits); ids equal to padding_id (-1: none) or outside [0, vocab) are
+ * left out.  into 0: a new [vocab, dim] tensor; else added to that tensor's rows
+ * in place (rows of absent tokens are not touched), which *out then names. */
+TP_API int tp_token_embedding_backward(int64_t grad_out, int64_t ids, int64_t vocab, float scale, int64_t padding_id,
+                                       int64_t into, tp_handle* out);
+/* The same on device pointers: rows of `ld` (ldd, ldo) values, of which the
+ * first vocab (dim) are used and the rest left as they are; ids_kind 0 =
+ * float32 values, 1 = int32.  NULL outputs are not written.  No entry
+ * allocates; 4-byte alignment is enough for every buffer (16 for ws). */
+/* ids may be NULL with logp NULL; dlogits may be logits (in place, ldd == ld) */
+TP_API int tpk_token_logprobs(const float* logits, int64_t ld, const void* ids, int ids_kind, int64_t rows,
+                              int64_t vocab, int topk, float* logp, float* entropy, float* stats, int32_t* top_ids,
+                              float* top_logp);
+TP_API int tpk_token_logprobs_backward(const float* logits, int64_t ld, const void* ids, int ids_kind,
+                                       const float* stats, const float* entropy, const float* dlogp,
+                                       const float* dentropy, int64_t rows, int64_t vocab, float* dlogits,
+                                       int64_t ldd);
+TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, int ids_kind, int64_t n,
+                               int64_t vocab, int64_t dim, float scale, float* out, int64_t ldo);
+/* accumulate 0 writes every row of dtable, 1 adds to the rows of present
+ * tokens.  ws: at least the bytes that tpk_token_embedding_backward_ws names,
+ * used from the call's first kernel to its last; calls whose work may overlap
+ * on the GPU need one each. */
+TP_API int tpk_token_embedding_backward_ws(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes);
+TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const void* ids, int ids_kind, int64_t n,
+                                        int64_t vocab, int64_t dim, float scale, int64_t padding_id, int accumulate,
+                                        float* dtable, int64_t ld, void* ws, int64_t ws_bytes);
 
 /* ---- pointer-level optimizer kernels ---------------------------------------- */
 /* A tensor group is a device-side table of n (param, grad, state0, state1,
@@ -443,6 +517,16 @@ TP_API int tpk_adam_group(int64_t group, int kind, float lr, float beta1, float 
  * parts of their updated parameter there */
 TP_API int tpk_sgd_group(int64_t group, float lr, float momentum, float weight_decay, float dampening,
                          int nesterov, float grad_scale);
+/* tp_clip_grad_norm_multi over the group's gradients; norm_coef [2] is the
+ * caller's.  The group keeps the partial sums, so calls on one group must not
+ * overlap on the GPU (as its steps must not). */
+TP_API int tpk_group_clip_grad_norm(int64_t group, float norm_type, float max_norm, float* norm_coef);
+/* the norm and the coefficient only, for a step that scales on read */
+TP_API int tpk_group_grad_norm(int64_t group, float norm_type, float max_norm, float* norm_coef);
+/* tpk_adam_group with each gradient multiplied by *grad_scale (in HBM: norm_coef
+ * + 1 of the calls above) on read */
+TP_API int tpk_adam_group_scaled(int64_t group, int kind, float lr, float beta1, float beta2, float eps,
+                                 float weight_decay, float step_size, float inv_sqrt_bc2, const float* grad_scale);
 
 /* ---- pointer-level kernels for a step driver (no allocation) ----------------- */
 /* conv2d forward / data-gradient / weight-gradient on NCHW device buffers

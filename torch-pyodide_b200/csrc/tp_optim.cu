@@ -15,10 +15,13 @@
 // -ffp-contract=off (sqrt and division are IEEE-rounded in both).
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <unordered_map>
 
 #include "tp_core.h"
 #include "tp_launch.h"
+#include "tp_token.cuh"
 
 namespace tp {
 
@@ -57,10 +60,16 @@ __device__ __forceinline__ void adam_elem(float& p, float g, float& m, float& v,
   p = __fsub_rn(p, upd);
 }
 
-template <bool ADAMW>
+// SCALED: each gradient is multiplied by *gs on read (rounded once, as a pass
+// that scales the gradients in place rounds it).
+template <bool ADAMW, bool SCALED>
 __global__ void __launch_bounds__(256) k_adam_multi(const OptRow* __restrict__ rows, const OptChunk* __restrict__ chunks,
-                                                    int nchunks, AdamHP h) {
+                                                    int nchunks, AdamHP h, const float* __restrict__ gs) {
   ::tp::pdl_enter();
+  const float s = SCALED ? *gs : 1.0f;
+  auto scaled = [&](float4 g) {
+    return SCALED ? make_float4(__fmul_rn(g.x, s), __fmul_rn(g.y, s), __fmul_rn(g.z, s), __fmul_rn(g.w, s)) : g;
+  };
   for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
     OptChunk ch = chunks[c];
     OptRow r = rows[ch.row];
@@ -80,6 +89,8 @@ __global__ void __launch_bounds__(256) k_adam_multi(const OptRow* __restrict__ r
       int j = i + blockDim.x;
       float4 p0 = P4[i], g0 = G4[i], m0 = M4[i], v0 = V4[i];
       float4 p1 = P4[j], g1 = G4[j], m1 = M4[j], v1 = V4[j];
+      g0 = scaled(g0);
+      g1 = scaled(g1);
       adam_elem<ADAMW>(p0.x, g0.x, m0.x, v0.x, h);
       adam_elem<ADAMW>(p0.y, g0.y, m0.y, v0.y, h);
       adam_elem<ADAMW>(p0.z, g0.z, m0.z, v0.z, h);
@@ -92,7 +103,7 @@ __global__ void __launch_bounds__(256) k_adam_multi(const OptRow* __restrict__ r
       P4[j] = p1; M4[j] = m1; V4[j] = v1;
     }
     for (; i < len4; i += blockDim.x) {
-      float4 p0 = P4[i], g0 = G4[i], m0 = M4[i], v0 = V4[i];
+      float4 p0 = P4[i], g0 = scaled(G4[i]), m0 = M4[i], v0 = V4[i];
       adam_elem<ADAMW>(p0.x, g0.x, m0.x, v0.x, h);
       adam_elem<ADAMW>(p0.y, g0.y, m0.y, v0.y, h);
       adam_elem<ADAMW>(p0.z, g0.z, m0.z, v0.z, h);
@@ -101,7 +112,7 @@ __global__ void __launch_bounds__(256) k_adam_multi(const OptRow* __restrict__ r
     }
     for (int k = (len4 << 2) + threadIdx.x; k < len; k += blockDim.x) {
       float p = P[k], m = M[k], v = V[k];
-      adam_elem<ADAMW>(p, G[k], m, v, h);
+      adam_elem<ADAMW>(p, SCALED ? __fmul_rn(G[k], s) : G[k], m, v, h);
       P[k] = p; M[k] = m; V[k] = v;
     }
   }
@@ -314,6 +325,77 @@ __global__ void __launch_bounds__(256) k_ext_multi(const OptRow* __restrict__ ro
   }
 }
 
+// ---- the global gradient norm, and clipping ------------------------------------------
+// N = (sum |g|^p)^(1/p) over every gradient of the group, p in {1, 2, inf};
+// coef = min(1, max_norm / (N + 1e-6)), NaN if N is NaN (or both are infinite).
+// Every CTA walks its chunks (a fixed assignment) and leaves one f64 partial;
+// the next launch's CTAs each combine all partials in the same order, so equal
+// inputs give equal bits and no CTA waits for another.  Squares of f32 values
+// are exact in f64 and cannot overflow there.
+constexpr int NORM_MAX_CTAS = 1024;
+
+template <int P>  // 0: inf
+__device__ __forceinline__ double norm_fold(double a, double b) {
+  if (P != 0) return a + b;
+  return (isnan(a) || a > b) ? a : b;
+}
+template <int P>
+__device__ __forceinline__ double norm_term(float g) {
+  const double d = fabs((double)g);
+  return P == 2 ? d * d : d;
+}
+
+template <int P>
+__device__ double norm_block(double v, double* sh) {
+  for (int o = 16; o > 0; o >>= 1) v = norm_fold<P>(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = sh[0];
+  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v = norm_fold<P>(v, sh[w]);
+  return v;
+}
+
+template <int P>
+__global__ void __launch_bounds__(256) k_grad_norm(const OptRow* __restrict__ rows, const OptChunk* __restrict__ chunks,
+                                                   int nchunks, double* __restrict__ partials) {
+  ::tp::pdl_enter();
+  __shared__ double sh[8];
+  double acc = 0.0;
+  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+    const OptChunk ch = chunks[c];
+    const float* __restrict__ G = rows[ch.row].g + ch.start;
+    for (int i = threadIdx.x; i < ch.len; i += 256) acc = norm_fold<P>(acc, norm_term<P>(G[i]));
+  }
+  acc = norm_block<P>(acc, sh);
+  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+// The norm and the coefficient from the partials; SCALE: then every gradient
+// times the coefficient, left alone when it is exactly 1.
+template <int P, bool SCALE>
+__global__ void __launch_bounds__(256) k_grad_clip(const OptRow* __restrict__ rows, const OptChunk* __restrict__ chunks,
+                                                   int nchunks, const double* __restrict__ partials, int np,
+                                                   float max_norm, float* __restrict__ out) {
+  ::tp::pdl_enter();
+  __shared__ double sh[8];
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < np; i += 256) acc = norm_fold<P>(acc, partials[i]);
+  acc = norm_block<P>(acc, sh);
+  const double norm = P == 2 ? sqrt(acc) : acc;
+  const double q = (double)max_norm / (norm + 1e-6);
+  const float coef = (float)(q > 1.0 ? 1.0 : q);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    out[0] = (float)norm;
+    out[1] = coef;
+  }
+  if (!SCALE || coef == 1.0f) return;
+  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+    const OptChunk ch = chunks[c];
+    float* __restrict__ G = const_cast<float*>(rows[ch.row].g) + ch.start;
+    for (int i = threadIdx.x; i < ch.len; i += 256) G[i] = __fmul_rn(G[i], coef);
+  }
+}
+
 // ---- groups --------------------------------------------------------------------
 
 struct Group {
@@ -321,12 +403,15 @@ struct Group {
   OptChunk* chunks = nullptr;
   int nrows = 0;
   int nchunks = 0;
+  double* partials = nullptr;   // NORM_MAX_CTAS of the gradient norm (groups built with_norm)
+  bool grads_disjoint = true;   // no two rows share gradient memory: they can be scaled in place
 };
 
 static std::unordered_map<int64_t, Group> g_groups;
 static int64_t g_next_group = 1;
 
-static Group build_group(const std::vector<OptRow>& rows) {
+// with_norm: with the partials and the overlap check of the gradient norm
+static Group build_group(const std::vector<OptRow>& rows, bool with_norm = false) {
   std::vector<OptChunk> chunks;
   for (size_t r = 0; r < rows.size(); ++r) {
     const OptRow& x = rows[r];
@@ -344,11 +429,21 @@ static Group build_group(const std::vector<OptRow>& rows) {
   g.nrows = (int)rows.size();
   g.nchunks = (int)chunks.size();
   size_t rb = rows.size() * sizeof(OptRow), cb = chunks.size() * sizeof(OptChunk);
-  char* buf = (char*)dalloc(rb + cb + 16);
+  rb = (rb + 15) & ~(size_t)15;
+  char* buf = (char*)dalloc(rb + ((cb + 15) & ~(size_t)15) + (with_norm ? NORM_MAX_CTAS * sizeof(double) : 16));
   g.rows = (OptRow*)buf;
-  g.chunks = (OptChunk*)(buf + ((rb + 15) & ~(size_t)15));
+  g.chunks = (OptChunk*)(buf + rb);
+  g.partials = (double*)(buf + rb + ((cb + 15) & ~(size_t)15));
+  rb = rows.size() * sizeof(OptRow);
   if (rb) TP_CUDA(cudaMemcpyAsync(g.rows, rows.data(), rb, cudaMemcpyHostToDevice, stream()));
   if (cb) TP_CUDA(cudaMemcpyAsync(g.chunks, chunks.data(), cb, cudaMemcpyHostToDevice, stream()));
+  if (!with_norm) return g;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (const OptRow& x : rows)
+    if (x.n > 0) spans.emplace_back((uintptr_t)x.g, (uintptr_t)(x.g + x.n));
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) g.grads_disjoint = false;
   return g;
 }
 
@@ -371,10 +466,13 @@ static AdamHP adam_hp(float lr, float b1, float b2, float eps, float wd, float s
   return h;
 }
 
-void launch_adam_group(const Group& g, bool adamw, const AdamHP& h) {
+void launch_adam_group(const Group& g, bool adamw, const AdamHP& h, const float* gs = nullptr) {
   if (g.nchunks == 0) return;
-  if (adamw) TP_LAUNCH(k_adam_multi<true>, opt_grid(g.nchunks), 256, 0, g.rows, g.chunks, g.nchunks, h);
-  else TP_LAUNCH(k_adam_multi<false>, opt_grid(g.nchunks), 256, 0, g.rows, g.chunks, g.nchunks, h);
+  const unsigned grid = opt_grid(g.nchunks);
+  if (adamw && gs) TP_LAUNCH((k_adam_multi<true, true>), grid, 256, 0, g.rows, g.chunks, g.nchunks, h, gs);
+  else if (adamw) TP_LAUNCH((k_adam_multi<true, false>), grid, 256, 0, g.rows, g.chunks, g.nchunks, h, gs);
+  else if (gs) TP_LAUNCH((k_adam_multi<false, true>), grid, 256, 0, g.rows, g.chunks, g.nchunks, h, gs);
+  else TP_LAUNCH((k_adam_multi<false, false>), grid, 256, 0, g.rows, g.chunks, g.nchunks, h, gs);
 }
 
 void launch_sgd_group(const Group& g, const SgdHP& h) {
@@ -399,6 +497,41 @@ static void launch_ext_kind(int kind, const Group& g, const ExtHP& h) {
     default: launch_ext<EXT_RADAM>(g, h); break;
   }
 }
+
+// Codes of the norm: 2, 1 or inf.
+static int norm_code(float norm_type, float max_norm, const char* what) {
+  TP_REQUIRE(norm_type == 1.0f || norm_type == 2.0f || (std::isinf(norm_type) && norm_type > 0),
+             "%s: norm_type must be 1, 2 or inf, got %g", what, (double)norm_type);
+  TP_REQUIRE(max_norm >= 0.0f, "%s: max_norm must not be negative or NaN, got %g", what, (double)max_norm);
+  return std::isinf(norm_type) ? 0 : (int)norm_type;
+}
+
+template <int P>
+static void launch_norm(const Group& g, float max_norm, bool scale, float* out) {
+  const unsigned grid = opt_grid(g.nchunks);  // at most 4 CTAs per SM
+  const unsigned parts = grid < (unsigned)NORM_MAX_CTAS ? grid : (unsigned)NORM_MAX_CTAS;
+  TP_LAUNCH(k_grad_norm<P>, parts, 256, 0, g.rows, g.chunks, g.nchunks, g.partials);
+  if (scale) TP_LAUNCH((k_grad_clip<P, true>), grid, 256, 0, g.rows, g.chunks, g.nchunks, g.partials, (int)parts,
+                       max_norm, out);
+  else TP_LAUNCH((k_grad_clip<P, false>), 1, 256, 0, g.rows, g.chunks, g.nchunks, g.partials, (int)parts, max_norm,
+                 out);
+}
+
+// out[0] = the norm, out[1] = the coefficient; scale: the gradients too
+static void launch_grad_norm(const Group& g, int p, float max_norm, bool scale, float* out, const char* what) {
+  TP_REQUIRE(!scale || g.grads_disjoint, "%s: a gradient is listed twice (or two overlap); it would be scaled twice",
+             what);
+  if (p == 0) launch_norm<0>(g, max_norm, scale, out);
+  else if (p == 1) launch_norm<1>(g, max_norm, scale, out);
+  else launch_norm<2>(g, max_norm, scale, out);
+}
+
+// Frees a call's own group, also when the call throws.
+struct TempGroup {
+  Group g;
+  explicit TempGroup(const std::vector<OptRow>& rows) : g(build_group(rows, true)) {}
+  ~TempGroup() { cudaFreeAsync(g.rows, stream()); }
+};
 
 static std::vector<OptRow> rows_from_ids(const int64_t* p, const int64_t* gr, const int64_t* s0, const int64_t* s1,
                                          int n, const char* what) {
@@ -471,7 +604,7 @@ TP_API int tpk_group_create_lo(int n, float* const* params, float* const* grads,
     for (int i = 0; i < n; ++i)
       rows[i] = OptRow{params[i], grads[i], state0[i], state1 ? state1[i] : state0[i], lo ? lo[i] : nullptr,
                        numels[i]};
-    Group g = build_group(rows);
+    Group g = build_group(rows, true);
     int64_t id = g_next_group++;
     g_groups[id] = g;
     *out_group = id;
@@ -507,6 +640,82 @@ TP_API int tpk_sgd_group(int64_t group, float lr, float mom, float wd, float dam
     TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
     SgdHP h{lr, mom, wd, 1.0f - damp, grad_scale, mom != 0.0f ? 1 : 0, nesterov ? 1 : 0};
     launch_sgd_group(it->second, h);
+  });
+}
+
+TP_API int tpk_group_grad_norm(int64_t group, float norm_type, float max_norm, float* norm_coef) {
+  return guard([&] {
+    const char* what = "group_grad_norm";
+    const int p = norm_code(norm_type, max_norm, what);
+    TP_REQUIRE(norm_coef, "%s: norm_coef is NULL", what);
+    auto it = g_groups.find(group);
+    TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
+    launch_grad_norm(it->second, p, max_norm, false, norm_coef, what);
+  });
+}
+
+TP_API int tpk_group_clip_grad_norm(int64_t group, float norm_type, float max_norm, float* norm_coef) {
+  return guard([&] {
+    const char* what = "group_clip_grad_norm";
+    const int p = norm_code(norm_type, max_norm, what);
+    TP_REQUIRE(norm_coef, "%s: norm_coef is NULL", what);
+    auto it = g_groups.find(group);
+    TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
+    launch_grad_norm(it->second, p, max_norm, true, norm_coef, what);
+  });
+}
+
+TP_API int tpk_adam_group_scaled(int64_t group, int kind, float lr, float b1, float b2, float eps, float wd, float ss,
+                                 float isb, const float* grad_scale) {
+  return guard([&] {
+    TP_REQUIRE(kind == 0 || kind == 1, "adam_group_scaled: kind must be 0 (AdamW) or 1 (Adam), got %d", kind);
+    TP_REQUIRE(grad_scale, "adam_group_scaled: grad_scale is NULL");
+    auto it = g_groups.find(group);
+    TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
+    launch_adam_group(it->second, kind == 0, adam_hp(lr, b1, b2, eps, wd, ss, isb), grad_scale);
+  });
+}
+
+TP_API int tp_clip_grad_norm_multi(const int64_t* grads, int n, float norm_type, float max_norm, tp_handle* norm) {
+  return guard([&] {
+    const char* what = "clipGradNorm";
+    TP_REQUIRE(n >= 0, "%s: negative tensor count", what);
+    const int p = norm_code(norm_type, max_norm, what);
+    std::vector<OptRow> rows((size_t)n);
+    for (int i = 0; i < n; ++i) {
+      const Tensor& g = get(grads[i]);
+      TP_REQUIRE(g.phys == PHYS_F32, "%s: index tensors are not supported", what);
+      rows[i] = OptRow{g.f(), g.f(), g.f(), g.f(), nullptr, g.numel};
+    }
+    TempGroup t(rows);
+    Outputs o;
+    const int64_t two[1] = {2};
+    Tensor& out = o.add(make(two, 1, TP_FLOAT32));
+    launch_grad_norm(t.g, p, max_norm, true, out.f(), what);
+    o.emit_all({norm});
+  });
+}
+
+TP_API int tp_adam_clip_step_multi(int kind, const int64_t* p, const int64_t* g, const int64_t* m, const int64_t* v,
+                                   int n, float lr, float b1, float b2, float eps, float wd, float ss, float isb,
+                                   float max_norm, tp_handle* norm) {
+  return guard([&] {
+    const char* what = "adamClipStep";
+    TP_REQUIRE(n >= 0, "%s: negative tensor count", what);
+    TP_REQUIRE(kind == 0 || kind == 1, "%s: kind must be 0 (AdamW) or 1 (Adam), got %d", what, kind);
+    const int code = norm_code(2.0f, max_norm, what);
+    const std::vector<OptRow> rows = rows_from_ids(p, g, m, v, n, what);
+    for (int i = 0; i < n; ++i)
+      TP_REQUIRE(get(p[i]).phys == PHYS_F32 && get(g[i]).phys == PHYS_F32 && get(m[i]).phys == PHYS_F32 &&
+                     get(v[i]).phys == PHYS_F32,
+                 "%s: index tensors are not supported", what);
+    TempGroup t(rows);
+    Outputs o;
+    const int64_t two[1] = {2};
+    Tensor& out = o.add(make(two, 1, TP_FLOAT32));
+    launch_grad_norm(t.g, code, max_norm, false, out.f(), what);
+    launch_adam_group(t.g, kind == 0, adam_hp(lr, b1, b2, eps, wd, ss, isb), out.f() + 1);
+    o.emit_all({norm});
   });
 }
 

@@ -165,6 +165,20 @@ SIGNATURES: dict[str, list] = {
     "tp_adamw_step_multi": [I64P, I64P, I64P, I64P, INT] + [F32] * 7,
     "tp_adam_step_multi": [I64P, I64P, I64P, I64P, INT] + [F32] * 7,
     "tp_sgd_step_multi": [I64P, I64P, I64P, INT, F32, F32, F32, F32, INT],
+    "tp_clip_grad_norm_multi": [I64P, INT, F32, F32, HP],
+    "tp_adam_clip_step_multi": [INT, I64P, I64P, I64P, I64P, INT] + [F32] * 8 + [HP],
+    "tp_token_logprobs": [I64, I64, INT, HP, HP, HP, HP, HP],
+    "tp_token_logprobs_backward": [I64, I64, I64, I64, I64, I64, HP],
+    "tp_token_embedding": [I64, I64, F32, HP],
+    "tp_token_embedding_backward": [I64, I64, I64, F32, I64, I64, HP],
+    "tpk_token_logprobs": [P, I64, P, INT, I64, I64, INT, P, P, P, P, P],
+    "tpk_token_logprobs_backward": [P, I64, P, INT, P, P, P, P, I64, I64, P, I64],
+    "tpk_token_embedding": [P, I64, P, INT, I64, I64, I64, F32, P, I64],
+    "tpk_token_embedding_backward_ws": [I64, I64, I64, I64P],
+    "tpk_token_embedding_backward": [P, I64, P, INT, I64, I64, I64, F32, I64, INT, P, I64, P, I64],
+    "tpk_group_clip_grad_norm": [I64, F32, F32, P],
+    "tpk_group_grad_norm": [I64, F32, F32, P],
+    "tpk_adam_group_scaled": [I64, INT] + [F32] * 7 + [P],
     "tpk_group_create": [INT, PP, PP, PP, PP, I64P, I64P],
     "tpk_group_create_lo": [INT, PP, PP, PP, PP, PP, I64P, I64P],
     "tpk_group_destroy": [I64],

@@ -528,6 +528,49 @@ class CudaRuntime:
         check(self.lib.tp_radam_step_multi(i64arr(ps), i64arr(gs), i64arr(ms), i64arr(vs), len(ps), lr, b1, b2, eps,
                                            wd, stepSize, beta1PowT, beta2PowT, int(stepCount)))
 
+    # ---- the global gradient norm, and clipping ----------------------------------
+    def clipGradNormMulti(self, gs, maxNorm, normType=2.0):
+        """Scale the gradients in place so that their global norm (1, 2 or inf)
+        is at most maxNorm; returns [2]: the norm before, and the factor."""
+        return self._call(self.lib.tp_clip_grad_norm_multi, i64arr(gs), len(gs), float(normType), float(maxNorm))
+
+    def _adam_clip(self, kind, ps, gs, ms, vs, hyper, maxNorm):
+        if not len(ps) == len(gs) == len(ms) == len(vs):
+            raise _lib.TpError(-1, "adamClipStep: the tensor lists differ in length")
+        return self._call(self.lib.tp_adam_clip_step_multi, kind, i64arr(ps), i64arr(gs), i64arr(ms), i64arr(vs),
+                          len(ps), *hyper, float(maxNorm))
+
+    def adamWClipStepMulti(self, ps, gs, ms, vs, lr, b1, b2, eps, wd, stepSize, invSqrtBc2, maxNorm):
+        """adamWStepMulti on gradients clipped to maxNorm (2-norm) as they are
+        read; returns [2]: the norm and the factor."""
+        return self._adam_clip(0, ps, gs, ms, vs, (lr, b1, b2, eps, wd, stepSize, invSqrtBc2), maxNorm)
+
+    def adamClipStepMulti(self, ps, gs, ms, vs, lr, b1, b2, eps, wd, stepSize, invSqrtBc2, maxNorm):
+        return self._adam_clip(1, ps, gs, ms, vs, (lr, b1, b2, eps, wd, stepSize, invSqrtBc2), maxNorm)
+
+    # ---- token operators ----------------------------------------------------------
+    def tokenLogprobs(self, logits, ids, topk=0):
+        """[logp, entropy, stats] of the token ids under softmax(logits), and with
+        topk > 0 also [topIds, topLogp], the most likely tokens."""
+        hs = [Handle() for _ in range(5 if topk else 3)]
+        check(self.lib.tp_token_logprobs(int(logits), int(ids), int(topk), *[ctypes.byref(h) for h in hs],
+                                         *([None] * (5 - len(hs)))))
+        return [h.to_dict() for h in hs]
+
+    def tokenLogprobsBackward(self, dlogp, dentropy, logits, ids, stats, entropy):
+        """Gradient of the logits from those of logp and entropy (either may be None)."""
+        o = self._opt
+        return self._call(self.lib.tp_token_logprobs_backward, o(dlogp), o(dentropy), int(logits), int(ids),
+                          int(stats), int(entropy))
+
+    def tokenEmbedding(self, table, ids, scale=1.0):
+        return self._call(self.lib.tp_token_embedding, int(table), int(ids), float(scale))
+
+    def tokenEmbeddingBackward(self, go, ids, vocab, scale=1.0, paddingId=None, into=None):
+        """Gradient of the table [vocab, dim]; `into`: an existing one to add to."""
+        return self._call(self.lib.tp_token_embedding_backward, int(go), int(ids), int(vocab), float(scale),
+                          -1 if paddingId is None else int(paddingId), self._opt(into))
+
     # ---- conv2d with a device bias (no readback of the bias) ---------------------
     def conv2dDevBias(self, inp, weight, bias, stride, padding, dilation, groups):
         st, pd, dl = list(stride), list(padding), list(dilation)
