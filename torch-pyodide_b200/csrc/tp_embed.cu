@@ -2,70 +2,450 @@
 //
 //   out_i = scale * table[id_i]         dtable_v (+)= scale * sum over { i : id_i = v } of dout_i
 //
-// The sum runs in an order fixed by the positions alone (no float atomics), so
-// equal inputs give equal bits.
+// Both move bytes and add little: what bounds them is HBM.  The gradient's sum
+// runs in an order fixed by the positions alone (no float atomics), so equal
+// inputs give equal bits.
 #include <cuda_runtime.h>
 
 #include <climits>
 
 #include "tp_core.h"
+#include "tp_fastdiv.cuh"
 #include "tp_launch.h"
 #include "tp_token.cuh"
 
 namespace tp {
 
-__global__ void __launch_bounds__(256) k_embed(const float* table, int64_t ld, const void* ids, int kind, int64_t n,
-                                               int64_t V, int64_t D, float scale, float* out, int64_t ldo) {
+// A column of a row: 4 values where rows start on 16-byte boundaries, else 1.
+template <int VEC>
+struct Col;
+template <>
+struct Col<4> {
+  float4 v;
+  __device__ static Col zero() { return {make_float4(0.0f, 0.0f, 0.0f, 0.0f)}; }
+  __device__ __forceinline__ void add(const Col& o) { v.x += o.v.x, v.y += o.v.y, v.z += o.v.z, v.w += o.v.w; }
+  __device__ __forceinline__ Col times(float s) const { return {make_float4(v.x * s, v.y * s, v.z * s, v.w * s)}; }
+  __device__ static Col load(const float* p, int64_t c) { return {*(reinterpret_cast<const float4*>(p) + c)}; }
+  __device__ void store(float* p, int64_t c) const { *(reinterpret_cast<float4*>(p) + c) = v; }
+};
+template <>
+struct Col<1> {
+  float v;
+  __device__ static Col zero() { return {0.0f}; }
+  __device__ __forceinline__ void add(const Col& o) { v += o.v; }
+  __device__ __forceinline__ Col times(float s) const { return {v * s}; }
+  __device__ static Col load(const float* p, int64_t c) { return {p[c]}; }
+  __device__ void store(float* p, int64_t c) const { p[c] = v; }
+};
+
+// CTAs of 128 threads, `tx` across a row's columns and the rest across rows.
+constexpr int EMB_NT = 128;
+static int block_cols(int64_t cols) {
+  int tx = 1;
+  while (tx < EMB_NT && tx < cols) tx *= 2;
+  return tx;
+}
+
+// ---- lookup ---------------------------------------------------------------------------
+constexpr int EMB_U = 4;  // columns per thread, loaded before the first is stored
+
+template <int VEC>
+__global__ void __launch_bounds__(EMB_NT) k_embed(const float* __restrict__ table, int64_t ld,
+                                                  const void* __restrict__ ids, int kind, int64_t n, int64_t V,
+                                                  int64_t cols, int chunks, float scale, float* __restrict__ out,
+                                                  int64_t ldo) {
   ::tp::pdl_enter();
-  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
-    const int64_t v = token_id(ids, kind, i);
-    const bool in = v >= 0 && v < V;
-    for (int64_t d = threadIdx.x; d < D; d += 256) out[i * ldo + d] = in ? table[v * ld + d] * scale : NAN;
+  const int64_t group = blockIdx.x / chunks;
+  const int64_t i = group * blockDim.y + threadIdx.y;
+  const int64_t c0 = (int64_t)(blockIdx.x - group * chunks) * EMB_U * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t v = token_id(ids, kind, i);
+  const bool in = v >= 0 && v < V;
+  const float* src = table + v * ld;
+  float* dst = out + i * ldo;
+  Col<VEC> x[EMB_U];
+#pragma unroll
+  for (int u = 0; u < EMB_U; ++u) {
+    const int64_t c = c0 + u * (int)blockDim.x;
+    if (in && c < cols) x[u] = Col<VEC>::load(src, c);
+  }
+#pragma unroll
+  for (int u = 0; u < EMB_U; ++u) {
+    const int64_t c = c0 + u * (int)blockDim.x;
+    if (c < cols) (in ? x[u].times(scale) : Col<VEC>::zero().times(NAN)).store(dst, c);
   }
 }
 
+// ---- gradient of a few tokens ---------------------------------------------------------
 // One CTA per (position, 256 columns): the first position of a token sums all
-// of them, in order.
-__global__ void __launch_bounds__(256) k_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
-                                                   int64_t n, int64_t V, int64_t D, float scale, int64_t pad,
-                                                   int accumulate, float* dtable, int64_t ld) {
+// of them, in order.  Reads the ids n times over, which for few is less than
+// sorting them costs.
+__global__ void __launch_bounds__(256) k_embed_bwd_few(const float* __restrict__ dout, int64_t ldo,
+                                                       const void* __restrict__ ids, int kind, int n, int64_t V,
+                                                       int64_t D, int chunks, float scale, int64_t pad,
+                                                       float* __restrict__ dtable, int64_t ld) {
   ::tp::pdl_enter();
   __shared__ uint32_t hit[8];
-  const int64_t i = blockIdx.x, d = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int i = blockIdx.x / chunks;
+  const int64_t d = (int64_t)(blockIdx.x - i * chunks) * 256 + threadIdx.x;
   const int64_t v = token_id(ids, kind, i);
   if (v < 0 || v >= V || v == pad) return;
   bool earlier = false;
-  for (int64_t j = threadIdx.x; j < i; j += 256) earlier |= token_id(ids, kind, j) == v;
+  for (int j = threadIdx.x; j < i; j += 256) earlier |= token_id(ids, kind, j) == v;
   if (__syncthreads_or(earlier)) return;
   float acc = 0.0f;
-  for (int64_t j0 = i; j0 < n; j0 += 256) {
-    const int64_t j = j0 + threadIdx.x;
+  for (int j0 = i; j0 < n; j0 += 256) {
+    const int j = j0 + threadIdx.x;
     const uint32_t b = __ballot_sync(0xffffffffu, j < n && token_id(ids, kind, j) == v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) hit[threadIdx.x >> 5] = b;
     __syncthreads();
+    float part = 0.0f;  // chains of at most 256 additions, then of n / 256
     for (int w = 0; w < 8; ++w)
       for (uint32_t q = hit[w]; q; q &= q - 1)
-        if (d < D) acc += dout[(j0 + 32 * w + __ffs(q) - 1) * ldo + d];
+        if (d < D) part += dout[(int64_t)(j0 + 32 * w + __ffs(q) - 1) * ldo + d];
+    acc += part;
   }
-  if (d < D) dtable[v * ld + d] = accumulate ? dtable[v * ld + d] + acc * scale : acc * scale;
+  if (d < D) dtable[v * ld + d] += acc * scale;
+}
+
+// ---- gradient of many tokens: positions sorted by token, then summed -----------------------
+// Sorting is one launch of CTAs that share nothing.  Token v belongs to CTA
+// v mod G, as its token v / G (neighbouring ids, of like frequency, go to
+// different CTAs).  Each CTA reads all ids: it counts those of the CTAs before
+// it, which is where its own begin, and the tokens of its own per warp; after a
+// scan over (token, warp) the warps place their positions in order.  A position
+// and its token are written per valid id, the start of each token's run per
+// token.  (Reading all ids G times is n G 4 bytes from L2; the rows they stand for
+// are n D 4 bytes from HBM.)
+constexpr int SORT_NT = 1024;
+constexpr int SORT_WARPS = SORT_NT / 32;
+constexpr int SORT_TOKENS = 512;          // tokens of one CTA, at most
+constexpr int SORT_WORDS = 32768;         // positions / 32 whose hits are kept in shared memory
+
+struct EmbedSort {
+  FastDiv ctas;   // G
+  int per;        // tokens of one CTA, W
+  int64_t n;
+  int V, pad, kind;
+  const void* ids;
+  int32_t* start;  // [G W + 1]: where the run of key owner * W + local starts; the last: how many positions there are
+  int32_t* pos;    // [n]
+  int32_t* tok;    // [n]
+  __device__ __forceinline__ bool valid(int v) const { return v >= 0 && v < V && v != pad; }
+  __device__ __forceinline__ int key(int v) const {
+    const int q = (int)ctas.div((uint32_t)v);
+    return (v - q * (int)ctas.d) * per + q;
+  }
+  __device__ __forceinline__ int total() const { return start[(int64_t)ctas.d * per]; }
+};
+
+__global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
+  ::tp::pdl_enter();
+  extern __shared__ int32_t sort_sm[];
+  __shared__ int32_t sh[SORT_WARPS];
+  const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  int32_t* count = sort_sm;                                  // [warps][W]
+  uint32_t* words = (uint32_t*)(sort_sm + SORT_WARPS * W);   // hits of 32 positions each
+  const int64_t nwords = (e.n + 31) >> 5;
+  const bool kept = nwords <= SORT_WORDS;
+  const int64_t per = (nwords + SORT_WARPS - 1) / SORT_WARPS;  // words of one warp: neighbours, so that order is kept
+  const int64_t w0 = per * w < nwords ? per * w : nwords, w1 = w0 + per < nwords ? w0 + per : nwords;
+  for (int i = t; i < SORT_WARPS * W; i += SORT_NT) count[i] = 0;
+  __syncthreads();
+  auto token = [&](int64_t word) {
+    const int64_t p = word * 32 + lane;
+    return word < w1 && p < e.n ? token_id(e.ids, e.kind, p) : -1;
+  };
+  int less = 0;
+  for (int64_t i = w0; i < w1; i += 4) {
+    int v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = token(i + q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool ok = e.valid(v[q]);
+      const int local = (int)e.ctas.div(ok ? (uint32_t)v[q] : 0u), owner = v[q] - local * (int)e.ctas.d;
+      less += ok && owner < me;
+      const bool hit = ok && owner == me;
+      if (hit) atomicAdd(&count[w * W + local], 1);
+      const uint32_t b = __ballot_sync(0xffffffffu, hit);
+      if (kept && lane == 0 && i + q < w1) words[i + q] = b;
+    }
+  }
+  for (int o = 16; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
+  if (lane == 0) sh[w] = less;
+  __syncthreads();
+  int base = 0;
+  for (int i = 0; i < SORT_WARPS; ++i) base += sh[i];
+  __syncthreads();
+  // one thread per token: its warps' counts become offsets within the token
+  int c = 0;
+  if (t < W)
+    for (int i = 0; i < SORT_WARPS; ++i) {
+      const int k = count[i * W + t];
+      count[i * W + t] = c;
+      c += k;
+    }
+  int incl = c;  // scan over the tokens
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) sh[w] = incl;
+  __syncthreads();
+  int first = base + incl - c;
+  for (int i = 0; i < w; ++i) first += sh[i];
+  if (t < W) {
+    e.start[(int64_t)me * W + t] = first;
+    for (int i = 0; i < SORT_WARPS; ++i) count[i * W + t] += first;
+    if (me == (int)gridDim.x - 1 && t == W - 1) e.start[(int64_t)gridDim.x * W] = first + c;
+  }
+  __syncthreads();
+  auto place = [&](int64_t word, uint32_t b) {
+    if (!(b >> lane & 1)) return;
+    const int64_t p = word * 32 + lane;
+    const int v = token_id(e.ids, e.kind, p), local = (int)e.ctas.div((uint32_t)v);
+    const uint32_t peers = __match_any_sync(b, local);
+    const int rank = __popc(peers & ((1u << lane) - 1)), at = count[w * W + local];
+    __syncwarp(b);
+    if (rank == 0) count[w * W + local] = at + __popc(peers);
+    __syncwarp(b);
+    e.pos[at + rank] = (int32_t)p;
+    e.tok[at + rank] = v;
+  };
+  if (kept) {
+    for (int64_t i = w0; i < w1; i += 32) {
+      const uint32_t mine = i + lane < w1 ? words[i + lane] : 0u;
+      for (uint32_t some = __ballot_sync(0xffffffffu, mine != 0u); some; some &= some - 1) {
+        const int j = __ffs(some) - 1;
+        place(i + j, __shfl_sync(0xffffffffu, mine, j));
+        __syncwarp();
+      }
+    }
+  } else {
+    for (int64_t i = w0; i < w1; ++i) {
+      const int v = token(i);
+      const bool ok = e.valid(v);
+      const uint32_t b = __ballot_sync(0xffffffffu, ok && (int)e.ctas.mod(ok ? (uint32_t)v : 0u) == me);
+      place(i, b);
+      __syncwarp();
+    }
+  }
+}
+
+// Tiles of SUM_T sorted positions are summed each by itself, whatever tokens
+// they hold, so a frequent token takes no longer than many rare ones.  A run of
+// one token that lies within the tile goes to its row; the part of a run that
+// came in from the tile before goes to the tile's partial 0, the start of one
+// that goes on to partial 1 (a run that does both is the former).
+constexpr int SUM_T = 64;
+constexpr int SUM_ZERO = 4;  // rows without a token that a thread clears
+
+template <int VEC, bool ACC>
+__global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const float* __restrict__ dout, int64_t ldo,
+                                                      int64_t cols, int chunks, int64_t tile_ctas, float scale,
+                                                      float* __restrict__ dtable, int64_t ld,
+                                                      float* __restrict__ partial, int64_t ldp) {
+  ::tp::pdl_enter();
+  const int64_t group = blockIdx.x / chunks;
+  const int64_t c = (int64_t)(blockIdx.x - group * chunks) * blockDim.x + threadIdx.x;
+  if (c >= cols) return;
+  if (group >= tile_ctas) {  // rows whose token is absent
+    const int64_t v0 = ((group - tile_ctas) * blockDim.y + threadIdx.y) * SUM_ZERO;
+#pragma unroll
+    for (int r = 0; r < SUM_ZERO; ++r) {
+      const int64_t v = v0 + r;
+      if (v >= e.V) return;
+      const int k = e.key((int)v);
+      if (e.start[k] == e.start[k + 1]) Col<VEC>::zero().store(dtable + v * ld, c);
+    }
+    return;
+  }
+  const int64_t tile = group * blockDim.y + threadIdx.y;
+  const int m = e.total();
+  if (tile * SUM_T >= m) return;
+  const int s0 = (int)(tile * SUM_T), s1 = m - s0 < SUM_T ? m : s0 + SUM_T;
+  int cur = e.tok[s0];
+  bool came_in = s0 > 0 && e.tok[s0 - 1] == cur;
+  float* part = partial + 2 * tile * ldp;
+  Col<VEC> acc = Col<VEC>::zero();
+  auto flush = [&]() {
+    if (came_in) {
+      acc.store(part, c);
+    } else {
+      float* row = dtable + (int64_t)cur * ld;
+      Col<VEC> r = acc.times(scale);
+      if (ACC) r.add(Col<VEC>::load(row, c));
+      r.store(row, c);
+    }
+  };
+  for (int s = s0; s < s1; s += 8) {
+    int tok[8];
+    Col<VEC> x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s + k < s1) {
+        tok[k] = e.tok[s + k];
+        x[k] = Col<VEC>::load(dout + (int64_t)e.pos[s + k] * ldo, c);
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (s + k < s1) {
+        if (tok[k] != cur) {
+          flush();
+          cur = tok[k];
+          came_in = false;
+          acc = Col<VEC>::zero();
+        }
+        acc.add(x[k]);
+      }
+  }
+  if (!came_in && s1 < m && e.tok[s1] == cur) acc.store(part + ldp, c);
+  else flush();
+}
+
+// Runs that cross tiles: the tile a run starts in adds up its partial 1 and the
+// partials 0 of the tiles after it, in f64: eight threads take every eighth,
+// and their sums are added in order.  A CTA looks through 32 tiles for such starts.
+constexpr int JOIN_COLS = 32, JOIN_ROWS = 8;
+
+template <bool ACC>
+__global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) k_embed_join(const EmbedSort e, int64_t D, int chunks,
+                                                                     float scale, float* __restrict__ dtable,
+                                                                     int64_t ld, const float* __restrict__ partial,
+                                                                     int64_t ldp) {
+  ::tp::pdl_enter();
+  __shared__ double sh[JOIN_ROWS][JOIN_COLS];
+  const int64_t group = blockIdx.x / chunks;
+  const int64_t c = (int64_t)(blockIdx.x - group * chunks) * JOIN_COLS + threadIdx.x;
+  const int m = e.total();
+  const int64_t mine = group * 32 + threadIdx.x;  // every warp looks at the same 32 tiles
+  bool starts = false;
+  if ((mine + 1) * SUM_T < m) {
+    const int s1 = (int)((mine + 1) * SUM_T), v = e.tok[s1 - 1];
+    starts = e.tok[s1] == v && e.start[e.key(v)] >= mine * SUM_T;
+  }
+  for (uint32_t some = __ballot_sync(0xffffffffu, starts); some; some &= some - 1) {
+    const int64_t tile = group * 32 + __ffs(some) - 1;
+    const int v = e.tok[tile * SUM_T + SUM_T - 1];
+    const int64_t last = (e.start[e.key(v) + 1] - 1) / SUM_T;
+    double acc = 0.0;
+    if (c < D) {
+      if (threadIdx.y == 0) acc = partial[(2 * tile + 1) * ldp + c];
+#pragma unroll 8
+      for (int64_t k = tile + 1 + threadIdx.y; k <= last; k += JOIN_ROWS) acc += partial[2 * k * ldp + c];
+    }
+    sh[threadIdx.y][threadIdx.x] = acc;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < D) {
+      for (int r = 1; r < JOIN_ROWS; ++r) acc += sh[r][threadIdx.x];
+      float* row = dtable + (int64_t)v * ld;
+      const float g = (float)(acc * scale);
+      row[c] = ACC ? row[c] + g : g;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------
+static bool aligned_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
+
+static unsigned grid_of(int64_t groups, int64_t chunks, const char* what) {
+  TP_REQUIRE(groups <= INT_MAX / chunks, "%s: too many tokens, rows or columns for one launch", what);
+  return (unsigned)(groups * chunks);
 }
 
 void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
                   float scale, float* out, int64_t ldo) {
   if (n == 0 || D == 0) return;
-  TP_LAUNCH(k_embed, (unsigned)(n < 65536 ? n : 65536), 256, 0, table, ld, ids, kind, n, V, D, scale, out, ldo);
+  const bool vec = D % 4 == 0 && aligned_rows(table, ld) && aligned_rows(out, ldo);
+  const int64_t cols = vec ? D / 4 : D;
+  const int tx = block_cols((cols + EMB_U - 1) / EMB_U), ty = EMB_NT / tx;
+  const int chunks = (int)((cols + EMB_U * tx - 1) / (EMB_U * tx));
+  const unsigned grid = grid_of((n + ty - 1) / ty, chunks, "token_embedding");
+  if (vec) TP_LAUNCH(k_embed<4>, grid, dim3(tx, ty), 0, table, ld, ids, kind, n, V, cols, chunks, scale, out, ldo);
+  else TP_LAUNCH(k_embed<1>, grid, dim3(tx, ty), 0, table, ld, ids, kind, n, V, cols, chunks, scale, out, ldo);
 }
 
-int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return 16; }
+// Up to this many tokens are added to an existing gradient without sorting.
+constexpr int64_t EMB_FEW = 2048;
+
+struct EmbedPlan {
+  int64_t ctas, per, start, pos, tok, partial, ldp, bytes, tiles;
+  EmbedPlan(int64_t n, int64_t V, int64_t D) {
+    const int64_t sms = 148, waves = (V + sms * SORT_TOKENS - 1) / (sms * SORT_TOKENS);
+    ctas = V < sms * waves ? V : sms * waves;
+    per = (V + ctas - 1) / ctas;
+    tiles = (n + SUM_T - 1) / SUM_T;
+    ldp = (D + 3) / 4 * 4;
+    auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
+    start = 0;
+    pos = start + up((ctas * per + 1) * 4);
+    tok = pos + up(n * 4);
+    partial = tok + up(n * 4);
+    bytes = partial + 2 * tiles * ldp * 4;
+  }
+};
+
+int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return EmbedPlan(n, V, D).bytes; }
+
+template <int VEC, bool ACC>
+static void launch_sum(const EmbedPlan& p, const EmbedSort& e, const float* dout, int64_t ldo, int64_t D, float scale,
+                       float* dtable, int64_t ld, float* partial) {
+  const char* what = "token_embedding_backward";
+  const int64_t cols = VEC == 4 ? D / 4 : D;
+  const int tx = block_cols(cols), ty = EMB_NT / tx;
+  const int chunks = (int)((cols + tx - 1) / tx);
+  const int64_t tile_ctas = (p.tiles + ty - 1) / ty;
+  const int64_t zero_ctas = ACC ? 0 : ((int64_t)e.V + ty * SUM_ZERO - 1) / (ty * SUM_ZERO);
+  const unsigned grid = grid_of(tile_ctas + zero_ctas, chunks, what);
+  if (grid == 0) return;
+  TP_LAUNCH((k_embed_sum<VEC, ACC>), grid, dim3(tx, ty), 0, e, dout, ldo, cols, chunks, tile_ctas, scale, dtable, ld,
+            partial, p.ldp);
+  if (p.tiles < 2) return;  // nothing crosses
+  const int jchunks = (int)((D + JOIN_COLS - 1) / JOIN_COLS);
+  TP_LAUNCH(k_embed_join<ACC>, grid_of((p.tiles + 31) / 32, jchunks, what), dim3(JOIN_COLS, JOIN_ROWS), 0, e, D,
+            jchunks, scale, dtable, ld, partial, p.ldp);
+}
 
 void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
                       float scale, int64_t pad, bool accumulate, float* dtable, int64_t ld, void* ws) {
-  if (!accumulate)
-    TP_CUDA(cudaMemset2DAsync(dtable, (size_t)ld * 4, 0, (size_t)D * 4, (size_t)V, stream()));
-  if (n == 0 || D == 0) return;
-  TP_LAUNCH(k_embed_bwd, dim3((unsigned)n, (unsigned)((D + 255) / 256)), 256, 0, dout, ldo, ids, kind, n, V, D, scale,
-            pad, accumulate ? 1 : 0, dtable, ld);
+  if (D == 0 || (n == 0 && accumulate)) return;
+  if (accumulate && n <= EMB_FEW) {
+    const int chunks = (int)((D + 255) / 256);
+    TP_LAUNCH(k_embed_bwd_few, grid_of(n, chunks, "token_embedding_backward"), 256, 0, dout, ldo, ids, kind, (int)n, V,
+              D, chunks, scale, pad, dtable, ld);
+    return;
+  }
+  const EmbedPlan p(n, V, D);
+  char* base = (char*)ws;
+  EmbedSort e;
+  e.ctas = fast_div((uint32_t)p.ctas);
+  e.per = (int)p.per;
+  e.n = n;
+  e.V = (int)V;
+  e.pad = (int)pad;
+  e.kind = kind;
+  e.ids = ids;
+  e.start = (int32_t*)(base + p.start);
+  e.pos = (int32_t*)(base + p.pos);
+  e.tok = (int32_t*)(base + p.tok);
+  float* partial = (float*)(base + p.partial);
+  const int64_t words = (n + 31) / 32;
+  const size_t smem = (size_t)(SORT_WARPS * p.per + (words <= SORT_WORDS ? words : 0)) * 4;
+  static bool raised = false;
+  if (!raised) {  // 64 KB of counts and 128 KB of hits at most
+    TP_CUDA(cudaFuncSetAttribute(k_embed_sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (SORT_WARPS * SORT_TOKENS + SORT_WORDS) * 4));
+    raised = true;
+  }
+  TP_LAUNCH(k_embed_sort, (unsigned)p.ctas, SORT_NT, smem, e);
+  const bool vec = D % 4 == 0 && aligned_rows(dout, ldo) && aligned_rows(dtable, ld);
+  if (vec && accumulate) launch_sum<4, true>(p, e, dout, ldo, D, scale, dtable, ld, partial);
+  else if (vec) launch_sum<4, false>(p, e, dout, ldo, D, scale, dtable, ld, partial);
+  else if (accumulate) launch_sum<1, true>(p, e, dout, ldo, D, scale, dtable, ld, partial);
+  else launch_sum<1, false>(p, e, dout, ldo, D, scale, dtable, ld, partial);
 }
 
 static void check_embed(int64_t n, int64_t V, int64_t D, int64_t ld, int64_t ldo, const char* what) {
