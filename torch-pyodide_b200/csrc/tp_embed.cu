@@ -122,6 +122,7 @@ constexpr int SORT_NT = 1024;
 constexpr int SORT_WARPS = SORT_NT / 32;
 constexpr int SORT_TOKENS = 512;          // tokens of one CTA, at most
 constexpr int SORT_WORDS = 32768;         // positions / 32 whose hits are kept in shared memory
+constexpr int SORT_U = 16;                // ids of a thread in flight
 
 struct EmbedSort {
   FastDiv ctas;   // G
@@ -143,7 +144,7 @@ struct EmbedSort {
 __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   ::tp::pdl_enter();
   extern __shared__ int32_t sort_sm[];
-  __shared__ int32_t sh[SORT_WARPS];
+  __shared__ int32_t sh[SORT_WARPS], hits[SORT_WARPS][64];
   const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
   int32_t* count = sort_sm;                                  // [warps][W]
   uint32_t* words = (uint32_t*)(sort_sm + SORT_WARPS * W);   // hits of 32 positions each
@@ -158,12 +159,12 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
     return word < w1 && p < e.n ? token_id(e.ids, e.kind, p) : -1;
   };
   int less = 0;
-  for (int64_t i = w0; i < w1; i += 4) {
-    int v[4];
+  for (int64_t i = w0; i < w1; i += SORT_U) {
+    int v[SORT_U];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = token(i + q);
+    for (int q = 0; q < SORT_U; ++q) v[q] = token(i + q);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < SORT_U; ++q) {
       const bool ok = e.valid(v[q]);
       const int local = (int)e.ctas.div(ok ? (uint32_t)v[q] : 0u), owner = v[q] - local * (int)e.ctas.d;
       less += ok && owner < me;
@@ -179,14 +180,14 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   int base = 0;
   for (int i = 0; i < SORT_WARPS; ++i) base += sh[i];
   __syncthreads();
-  // one thread per token: its warps' counts become offsets within the token
-  int c = 0;
+  // one thread per token: its warps' counts become the places of their positions
+  int k[SORT_WARPS], c = 0;
   if (t < W)
-    for (int i = 0; i < SORT_WARPS; ++i) {
-      const int k = count[i * W + t];
-      count[i * W + t] = c;
-      c += k;
-    }
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) k[i] = count[i * W + t];
+  if (t < W)
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) c += k[i];
   int incl = c;  // scan over the tokens
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, incl, o);
@@ -198,55 +199,76 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   for (int i = 0; i < w; ++i) first += sh[i];
   if (t < W) {
     e.start[(int64_t)me * W + t] = first;
-    for (int i = 0; i < SORT_WARPS; ++i) count[i * W + t] += first;
+    int at = first;
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) {
+      count[i * W + t] = at;
+      at += k[i];
+    }
     if (me == (int)gridDim.x - 1 && t == W - 1) e.start[(int64_t)gridDim.x * W] = first + c;
   }
   __syncthreads();
-  auto place = [&](int64_t word, uint32_t b) {
-    if (!(b >> lane & 1)) return;
-    const int64_t p = word * 32 + lane;
-    const int v = token_id(e.ids, e.kind, p), local = (int)e.ctas.div((uint32_t)v);
-    const uint32_t peers = __match_any_sync(b, local);
-    const int rank = __popc(peers & ((1u << lane) - 1)), at = count[w * W + local];
-    __syncwarp(b);
-    if (rank == 0) count[w * W + local] = at + __popc(peers);
-    __syncwarp(b);
-    e.pos[at + rank] = (int32_t)p;
-    e.tok[at + rank] = v;
+  // Positions of hits, in order, 32 at a time: a lane each.
+  int32_t* buf = hits[w];
+  int have = 0;
+  auto place = [&](int k) {  // the first k of buf
+    __syncwarp();
+    const uint32_t some = k == 32 ? 0xffffffffu : (1u << k) - 1;
+    if (lane < k) {
+      const int p = buf[lane], v = token_id(e.ids, e.kind, p), local = (int)e.ctas.div((uint32_t)v);
+      const uint32_t peers = __match_any_sync(some, local);
+      const int rank = __popc(peers & ((1u << lane) - 1)), at = count[w * W + local];
+      __syncwarp(some);
+      if (rank == 0) count[w * W + local] = at + __popc(peers);
+      e.pos[at + rank] = p;
+      e.tok[at + rank] = v;
+    }
+    __syncwarp();
+  };
+  auto take = [&](int64_t word, uint32_t b) {
+    if (b >> lane & 1) buf[have + __popc(b & ((1u << lane) - 1))] = (int32_t)(word * 32 + lane);
+    have += __popc(b);
+    if (have >= 32) {
+      place(32);
+      const int32_t rest = buf[32 + lane];
+      __syncwarp();
+      buf[lane] = rest;
+      have -= 32;
+      __syncwarp();
+    }
   };
   if (kept) {
     for (int64_t i = w0; i < w1; i += 32) {
       const uint32_t mine = i + lane < w1 ? words[i + lane] : 0u;
       for (uint32_t some = __ballot_sync(0xffffffffu, mine != 0u); some; some &= some - 1) {
         const int j = __ffs(some) - 1;
-        place(i + j, __shfl_sync(0xffffffffu, mine, j));
-        __syncwarp();
+        take(i + j, __shfl_sync(0xffffffffu, mine, j));
       }
     }
   } else {
     for (int64_t i = w0; i < w1; ++i) {
       const int v = token(i);
       const bool ok = e.valid(v);
-      const uint32_t b = __ballot_sync(0xffffffffu, ok && (int)e.ctas.mod(ok ? (uint32_t)v : 0u) == me);
-      place(i, b);
-      __syncwarp();
+      take(i, __ballot_sync(0xffffffffu, ok && (int)e.ctas.mod(ok ? (uint32_t)v : 0u) == me));
     }
   }
+  if (have) place(have);
 }
 
-// Tiles of SUM_T sorted positions are summed each by itself, whatever tokens
-// they hold, so a frequent token takes no longer than many rare ones.  A run of
-// one token that lies within the tile goes to its row; the part of a run that
-// came in from the tile before goes to the tile's partial 0, the start of one
-// that goes on to partial 1 (a run that does both is the former).
-constexpr int SUM_T = 64;
+// Tiles of SUM_T sorted positions are summed each by itself, so a frequent
+// token takes no longer than many rare ones.  A run (the positions of one token)
+// of at most SUM_RUN goes whole to the tile it starts in.  A longer one is cut
+// at the tiles' borders: what came in from the tile before is the tile's
+// partial 0, the start of what goes on its partial 1 (what does both, partial 0).
+constexpr int SUM_T = 64, SUM_RUN = 128;
 constexpr int SUM_ZERO = 4;  // rows without a token that a thread clears
 
 template <int VEC, bool ACC>
 __global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const float* __restrict__ dout, int64_t ldo,
-                                                      int64_t cols, int chunks, int64_t tile_ctas, float scale,
-                                                      float* __restrict__ dtable, int64_t ld,
-                                                      float* __restrict__ partial, int64_t ldp) {
+                                                      int64_t cols, int chunks, int64_t tiles, int64_t tile_ctas,
+                                                      float scale, float* __restrict__ dtable, int64_t ld,
+                                                      float* __restrict__ partial, int64_t ldp,
+                                                      int2* __restrict__ cut) {
   ::tp::pdl_enter();
   const int64_t group = blockIdx.x / chunks;
   const int64_t c = (int64_t)(blockIdx.x - group * chunks) * blockDim.x + threadIdx.x;
@@ -264,10 +286,35 @@ __global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const f
   }
   const int64_t tile = group * blockDim.y + threadIdx.y;
   const int m = e.total();
-  if (tile * SUM_T >= m) return;
-  const int s0 = (int)(tile * SUM_T), s1 = m - s0 < SUM_T ? m : s0 + SUM_T;
+  int2 starts = make_int2(-1, 0);  // the cut run that starts here: its token, its last tile
+  if (tile * SUM_T >= m) {
+    if (c == 0 && tile < tiles) cut[tile] = starts;
+    return;
+  }
+  const int s0 = (int)(tile * SUM_T);
+  int s1 = m - s0 < SUM_T ? m : s0 + SUM_T, from = s0;
   int cur = e.tok[s0];
-  bool came_in = s0 > 0 && e.tok[s0 - 1] == cur;
+  bool came_in = false, goes_on = false;
+  if (s0 > 0 && e.tok[s0 - 1] == cur) {
+    const int k = e.key(cur), end = e.start[k + 1];
+    if (end - e.start[k] > SUM_RUN) came_in = true;
+    else from = end;
+  }
+  if (s1 < m) {
+    const int v = e.tok[s1 - 1];
+    if (e.tok[s1] == v) {
+      const int k = e.key(v), end = e.start[k + 1];
+      if (end - e.start[k] > SUM_RUN) {
+        goes_on = true;
+        if (e.start[k] >= s0) starts = make_int2(v, (end - 1) / SUM_T);
+      } else if (e.start[k] >= s0) {
+        s1 = end;
+      }
+    }
+  }
+  if (c == 0) cut[tile] = starts;
+  if (from >= s1) return;  // all of it belongs to a run of the tile before
+  cur = e.tok[from];
   float* part = partial + 2 * tile * ldp;
   Col<VEC> acc = Col<VEC>::zero();
   auto flush = [&]() {
@@ -280,7 +327,7 @@ __global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const f
       r.store(row, c);
     }
   };
-  for (int s = s0; s < s1; s += 8) {
+  for (int s = from; s < s1; s += 8) {
     int tok[8];
     Col<VEC> x[8];
 #pragma unroll
@@ -301,17 +348,18 @@ __global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const f
         acc.add(x[k]);
       }
   }
-  if (!came_in && s1 < m && e.tok[s1] == cur) acc.store(part + ldp, c);
+  if (!came_in && goes_on) acc.store(part + ldp, c);
   else flush();
 }
 
-// Runs that cross tiles: the tile a run starts in adds up its partial 1 and the
+// The runs that were cut: the tile one starts in adds up its partial 1 and the
 // partials 0 of the tiles after it, in f64: eight threads take every eighth,
 // and their sums are added in order.  A CTA looks through 32 tiles for such starts.
 constexpr int JOIN_COLS = 32, JOIN_ROWS = 8;
 
 template <bool ACC>
-__global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) k_embed_join(const EmbedSort e, int64_t D, int chunks,
+__global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) k_embed_join(const int2* __restrict__ cut,
+                                                                     int64_t tiles, int64_t D, int chunks,
                                                                      float scale, float* __restrict__ dtable,
                                                                      int64_t ld, const float* __restrict__ partial,
                                                                      int64_t ldp) {
@@ -319,17 +367,12 @@ __global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) k_embed_join(const Embed
   __shared__ double sh[JOIN_ROWS][JOIN_COLS];
   const int64_t group = blockIdx.x / chunks;
   const int64_t c = (int64_t)(blockIdx.x - group * chunks) * JOIN_COLS + threadIdx.x;
-  const int m = e.total();
   const int64_t mine = group * 32 + threadIdx.x;  // every warp looks at the same 32 tiles
-  bool starts = false;
-  if ((mine + 1) * SUM_T < m) {
-    const int s1 = (int)((mine + 1) * SUM_T), v = e.tok[s1 - 1];
-    starts = e.tok[s1] == v && e.start[e.key(v)] >= mine * SUM_T;
-  }
-  for (uint32_t some = __ballot_sync(0xffffffffu, starts); some; some &= some - 1) {
-    const int64_t tile = group * 32 + __ffs(some) - 1;
-    const int v = e.tok[tile * SUM_T + SUM_T - 1];
-    const int64_t last = (e.start[e.key(v) + 1] - 1) / SUM_T;
+  const int2 run = mine < tiles ? cut[mine] : make_int2(-1, 0);
+  for (uint32_t some = __ballot_sync(0xffffffffu, run.x >= 0); some; some &= some - 1) {
+    const int which = __ffs(some) - 1;
+    const int64_t tile = group * 32 + which;
+    const int v = __shfl_sync(0xffffffffu, run.x, which), last = __shfl_sync(0xffffffffu, run.y, which);
     double acc = 0.0;
     if (c < D) {
       if (threadIdx.y == 0) acc = partial[(2 * tile + 1) * ldp + c];
@@ -372,7 +415,7 @@ void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int
 constexpr int64_t EMB_FEW = 2048;
 
 struct EmbedPlan {
-  int64_t ctas, per, start, pos, tok, partial, ldp, bytes, tiles;
+  int64_t ctas, per, start, pos, tok, cut, partial, ldp, bytes, tiles;
   EmbedPlan(int64_t n, int64_t V, int64_t D) {
     const int64_t sms = 148, waves = (V + sms * SORT_TOKENS - 1) / (sms * SORT_TOKENS);
     ctas = V < sms * waves ? V : sms * waves;
@@ -383,7 +426,8 @@ struct EmbedPlan {
     start = 0;
     pos = start + up((ctas * per + 1) * 4);
     tok = pos + up(n * 4);
-    partial = tok + up(n * 4);
+    cut = tok + up(n * 4);
+    partial = cut + up(tiles * 8);
     bytes = partial + 2 * tiles * ldp * 4;
   }
 };
@@ -392,7 +436,7 @@ int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return EmbedPlan(n, V, D
 
 template <int VEC, bool ACC>
 static void launch_sum(const EmbedPlan& p, const EmbedSort& e, const float* dout, int64_t ldo, int64_t D, float scale,
-                       float* dtable, int64_t ld, float* partial) {
+                       float* dtable, int64_t ld, float* partial, int2* cut) {
   const char* what = "token_embedding_backward";
   const int64_t cols = VEC == 4 ? D / 4 : D;
   const int tx = block_cols(cols), ty = EMB_NT / tx;
@@ -401,12 +445,12 @@ static void launch_sum(const EmbedPlan& p, const EmbedSort& e, const float* dout
   const int64_t zero_ctas = ACC ? 0 : ((int64_t)e.V + ty * SUM_ZERO - 1) / (ty * SUM_ZERO);
   const unsigned grid = grid_of(tile_ctas + zero_ctas, chunks, what);
   if (grid == 0) return;
-  TP_LAUNCH((k_embed_sum<VEC, ACC>), grid, dim3(tx, ty), 0, e, dout, ldo, cols, chunks, tile_ctas, scale, dtable, ld,
-            partial, p.ldp);
+  TP_LAUNCH((k_embed_sum<VEC, ACC>), grid, dim3(tx, ty), 0, e, dout, ldo, cols, chunks, p.tiles, tile_ctas, scale,
+            dtable, ld, partial, p.ldp, cut);
   if (p.tiles < 2) return;  // nothing crosses
   const int jchunks = (int)((D + JOIN_COLS - 1) / JOIN_COLS);
-  TP_LAUNCH(k_embed_join<ACC>, grid_of((p.tiles + 31) / 32, jchunks, what), dim3(JOIN_COLS, JOIN_ROWS), 0, e, D,
-            jchunks, scale, dtable, ld, partial, p.ldp);
+  TP_LAUNCH(k_embed_join<ACC>, grid_of((p.tiles + 31) / 32, jchunks, what), dim3(JOIN_COLS, JOIN_ROWS), 0,
+            cut, p.tiles, D, jchunks, scale, dtable, ld, partial, p.ldp);
 }
 
 void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
@@ -432,6 +476,7 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   e.pos = (int32_t*)(base + p.pos);
   e.tok = (int32_t*)(base + p.tok);
   float* partial = (float*)(base + p.partial);
+  int2* cut = (int2*)(base + p.cut);
   const int64_t words = (n + 31) / 32;
   const size_t smem = (size_t)(SORT_WARPS * p.per + (words <= SORT_WORDS ? words : 0)) * 4;
   static bool raised = false;
@@ -442,10 +487,10 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   }
   TP_LAUNCH(k_embed_sort, (unsigned)p.ctas, SORT_NT, smem, e);
   const bool vec = D % 4 == 0 && aligned_rows(dout, ldo) && aligned_rows(dtable, ld);
-  if (vec && accumulate) launch_sum<4, true>(p, e, dout, ldo, D, scale, dtable, ld, partial);
-  else if (vec) launch_sum<4, false>(p, e, dout, ldo, D, scale, dtable, ld, partial);
-  else if (accumulate) launch_sum<1, true>(p, e, dout, ldo, D, scale, dtable, ld, partial);
-  else launch_sum<1, false>(p, e, dout, ldo, D, scale, dtable, ld, partial);
+  if (vec && accumulate) launch_sum<4, true>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
+  else if (vec) launch_sum<4, false>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
+  else if (accumulate) launch_sum<1, true>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
+  else launch_sum<1, false>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
 }
 
 static void check_embed(int64_t n, int64_t V, int64_t D, int64_t ld, int64_t ldo, const char* what) {

@@ -96,62 +96,103 @@ struct LpRow {
   }
 };
 
-// ---- short rows: one warp each, the row in registers -----------------------------------
-// Lane l holds the logits l + 32 k, k < N.  The alternatives are found one after
-// the other: the warp's largest value, the lowest index that has it, and the
-// lane that owned it looks for its next.
+// ---- short rows: a warp each, the row in registers ---------------------------------------
+// A warp takes `per` rows (at most 8) one after the other; lane r keeps row r's
+// statistics, so that logarithms and stores are done for all rows at once.  Lane l
+// holds the logits l + 32 k, k < N, of the row at hand and the best two of them.
+// The alternatives are found one by one: the warp's largest value, the lowest
+// index that has it; the lane it came from puts its second best in its place, or
+// looks for it when that is used up too.
+constexpr int LP_ROWS = 8;
+
 template <int N, bool TOP>
 __global__ void __launch_bounds__(256) k_logprobs_warp(const float* __restrict__ x, int64_t ld,
-                                                       const void* __restrict__ ids, int kind, int64_t R, int V, int K,
-                                                       float* __restrict__ logp, float* __restrict__ entropy,
-                                                       float* __restrict__ stats, int32_t* __restrict__ top_ids,
-                                                       float* __restrict__ top_logp) {
+                                                       const void* __restrict__ ids, int kind, int64_t R, int V,
+                                                       int per, int K, float* __restrict__ logp,
+                                                       float* __restrict__ entropy, float* __restrict__ stats,
+                                                       int32_t* __restrict__ top_ids, float* __restrict__ top_logp) {
   ::tp::pdl_enter();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= R) return;
-  const float* __restrict__ xr = x + row * ld;
+  __shared__ unsigned long long keys[8][TOP ? LP_ROWS * LP_MAX_TOP : 1];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t row0 = ((int64_t)blockIdx.x * 8 + w) * per;
+  if (row0 >= R) return;
+  const int rows = R - row0 < per ? (int)(R - row0) : per;
   int t = -1;
-  if (logp && lane == 0) t = token_id(ids, kind, row);
-  float v[N];
+  if (logp && lane < rows) t = token_id(ids, kind, row0 + lane);
+  LpStat mine{-INFINITY, 0.0f, 0.0f};
+  for (int r = 0; r < rows; ++r) {
+    const float* __restrict__ xr = x + (row0 + r) * ld;
+    float v[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int i = lane + 32 * k;
-    v[k] = i < V ? xr[i] : -INFINITY;
-  }
-  const float xt = t >= 0 && t < V ? xr[t] : 0.0f;
-  LpStat s{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-  for (int k = 0; k < N; ++k) s.m = lp_max(s.m, v[k]);
-  float best = s.m;  // this lane's largest
-  for (int o = 16; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
-#pragma unroll
-  for (int k = 0; k < N; ++k) s.add(v[k]);
-  for (int o = 16; o > 0; o >>= 1) {
-    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
-    s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
-  }
-  const LpRow r(s);
-  if (lane == 0) r.write(s, row, V, t, xt, logp, entropy, stats);
-  for (int q = 0; TOP && q < K; ++q) {
-    const uint32_t o = r.bad || best == -INFINITY ? 0u : (uint32_t)(lp_key(best, 0) >> 32);
-    const uint32_t top = __reduce_max_sync(0xffffffffu, o);
-    uint32_t i = UINT_MAX;
-    if (o == top && top) {
-#pragma unroll
-      for (int k = N - 1; k >= 0; --k)
-        if (v[k] == best) i = lane + 32 * k;
+    for (int k = 0; k < N; ++k) {
+      const int i = lane + 32 * k;
+      v[k] = i < V ? xr[i] : -INFINITY;
     }
-    const uint32_t first = __reduce_min_sync(0xffffffffu, i);
-    if (i == first && top) {
-      best = -INFINITY;
+    LpStat s{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        if (first == (uint32_t)(lane + 32 * k)) v[k] = -INFINITY;
-        best = fmaxf(best, v[k]);
+    for (int k = 0; k < N; ++k) s.m = lp_max(s.m, v[k]);
+    for (int o = 16; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
+#pragma unroll
+    for (int k = 0; k < N; ++k) s.add(v[k]);
+    for (int o = 16; o > 0; o >>= 1) {
+      s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+      s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
+    }
+    if (lane == r) mine = s;
+    if (TOP) {
+      unsigned long long* out = keys[w] + r * K;
+      float b1 = -INFINITY, b2 = -INFINITY;
+      int i1 = 0, i2 = 0;
+      auto see = [&](float y, int k) {
+        if (y > b1) {
+          b2 = b1, i2 = i1;
+          b1 = y, i1 = k;
+        } else if (y > b2) {
+          b2 = y, i2 = k;
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < N; ++k) see(v[k], k);
+      bool second = true;
+      const bool odd = !(s.m < INFINITY);  // NaN or +inf in the row: no alternatives
+      for (int q = 0; q < K; ++q) {
+        const uint32_t o = odd || b1 == -INFINITY ? 0u : (uint32_t)(lp_key(b1, 0) >> 32);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, o);
+        const uint32_t i = o == top ? (uint32_t)(lane + 32 * i1) : UINT_MAX;
+        const uint32_t first = __reduce_min_sync(0xffffffffu, i);
+        if (lane == 0) out[q] = top ? (unsigned long long)top << 32 | (uint32_t)~first : 0ull;
+        if (top && i == first) {
+          if (second) {
+            b1 = b2, i1 = i2;
+            second = false;
+          } else {
+            const float y0 = b1;
+            const int k0 = i1;
+            b1 = b2 = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+              if (v[k] < y0 || (v[k] == y0 && k > k0)) see(v[k], k);
+            second = true;
+          }
+        }
       }
     }
-    if (lane == 0) r.write_top(top ? ((unsigned long long)top << 32 | (uint32_t)~first) : 0ull, row * K + q, top_ids, top_logp);
+  }
+  const LpRow a(mine);
+  if (lane < rows) {
+    const float xt = t >= 0 && t < V ? x[(row0 + lane) * ld + t] : 0.0f;
+    a.write(mine, row0 + lane, V, t, xt, logp, entropy, stats);
+  }
+  if (TOP) {
+    __syncwarp();
+    for (int e0 = 0; e0 < rows * K; e0 += 32) {
+      const int e = e0 + lane, r = e / K;
+      LpRow b = a;
+      b.bad = __shfl_sync(0xffffffffu, (int)a.bad, r & 31);
+      b.m = __shfl_sync(0xffffffffu, a.m, r & 31);
+      b.lnS = __shfl_sync(0xffffffffu, a.lnS, r & 31);
+      if (e < rows * K) b.write_top(keys[w][e], row0 * K + e, top_ids, top_logp);
+    }
   }
 }
 
@@ -577,20 +618,28 @@ constexpr int64_t LP_WARP_MAX = 1024;
 template <bool TOP>
 static void launch_logprobs_warp(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int V, int K,
                                  float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp) {
-  const unsigned grid = (unsigned)((R + 7) / 8);
-#define TP_LP_WARP(N)                                                                                            \
-  if (V <= 32 * N) {                                                                                             \
-    TP_LAUNCH((k_logprobs_warp<N, TOP>), grid, 256, 0, x, ld, ids, kind, R, V, K, logp, entropy, stats, top_ids, \
-              top_logp);                                                                                         \
-    return;                                                                                                      \
+  // one row per warp until there are warps for every scheduler several times over
+  int per = 1;
+  while (per < LP_ROWS && R >= (int64_t)sm_count() * 64 * 2 * per) per *= 2;
+  const unsigned grid = (unsigned)((R + 8 * per - 1) / (8 * per));
+#define TP_LP_WARP(N)                                                                                                 \
+  if (V <= 32 * N) {                                                                                                  \
+    TP_LAUNCH((k_logprobs_warp<N, TOP>), grid, 256, 0, x, ld, ids, kind, R, V, per, K, logp, entropy, stats, top_ids, \
+              top_logp);                                                                                              \
+    return;                                                                                                           \
   }
   TP_LP_WARP(1)
   TP_LP_WARP(2)
+  TP_LP_WARP(3)
   TP_LP_WARP(4)
+  TP_LP_WARP(6)
   TP_LP_WARP(8)
+  TP_LP_WARP(9)
   TP_LP_WARP(12)
   TP_LP_WARP(16)
+  TP_LP_WARP(20)
   TP_LP_WARP(24)
+  TP_LP_WARP(28)
   TP_LP_WARP(32)
 #undef TP_LP_WARP
 }

@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <unordered_map>
 
@@ -331,8 +332,13 @@ __global__ void __launch_bounds__(256) k_ext_multi(const OptRow* __restrict__ ro
 // Every CTA walks its chunks (a fixed assignment) and leaves one f64 partial;
 // the next launch's CTAs each combine all partials in the same order, so equal
 // inputs give equal bits and no CTA waits for another.  Squares of f32 values
-// are exact in f64 and cannot overflow there.
-constexpr int NORM_MAX_CTAS = 1024;
+// are exact in f64 and cannot overflow there.  The norm walks the chunks from
+// the last to the first, the pass after it (scaling, or the step) from the first:
+// what the norm read last is what that pass finds in L2.
+constexpr int NORM_MAX_CTAS = 1184;
+// A CTA takes a quarter of a chunk at a time: a few million gradients are then
+// still enough for every SM.
+constexpr int NORM_PART = (int)(OPT_CHUNK / 4);
 
 template <int P>  // 0: inf
 __device__ __forceinline__ double norm_fold(double a, double b) {
@@ -361,10 +367,24 @@ __global__ void __launch_bounds__(256) k_grad_norm(const OptRow* __restrict__ ro
   ::tp::pdl_enter();
   __shared__ double sh[8];
   double acc = 0.0;
-  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
-    const OptChunk ch = chunks[c];
-    const float* __restrict__ G = rows[ch.row].g + ch.start;
-    for (int i = threadIdx.x; i < ch.len; i += 256) acc = norm_fold<P>(acc, norm_term<P>(G[i]));
+  for (int c = 4 * nchunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    const OptChunk ch = chunks[c >> 2];
+    const int from = (c & 3) * NORM_PART;
+    if (from >= ch.len) continue;
+    const float* __restrict__ G = rows[ch.row].g + ch.start + from;
+    const float4* __restrict__ G4 = reinterpret_cast<const float4*>(G);
+    const int len = ch.len - from < NORM_PART ? ch.len - from : NORM_PART, len4 = len >> 2;
+    auto four = [&](float4 g) {
+      return norm_fold<P>(norm_fold<P>(norm_term<P>(g.x), norm_term<P>(g.y)),
+                          norm_fold<P>(norm_term<P>(g.z), norm_term<P>(g.w)));
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * 256 < len4; i += 4 * 256) {
+      const float4 a = G4[i], b = G4[i + 256], c4 = G4[i + 512], d = G4[i + 768];
+      acc = norm_fold<P>(acc, norm_fold<P>(norm_fold<P>(four(a), four(b)), norm_fold<P>(four(c4), four(d))));
+    }
+    for (; i < len4; i += 256) acc = norm_fold<P>(acc, four(G4[i]));
+    for (int k = (len4 << 2) + threadIdx.x; k < len; k += 256) acc = norm_fold<P>(acc, norm_term<P>(G[k]));
   }
   acc = norm_block<P>(acc, sh);
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
@@ -388,11 +408,27 @@ __global__ void __launch_bounds__(256) k_grad_clip(const OptRow* __restrict__ ro
     out[0] = (float)norm;
     out[1] = coef;
   }
-  if (!SCALE || coef == 1.0f) return;
-  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
-    const OptChunk ch = chunks[c];
-    float* __restrict__ G = const_cast<float*>(rows[ch.row].g) + ch.start;
-    for (int i = threadIdx.x; i < ch.len; i += 256) G[i] = __fmul_rn(G[i], coef);
+  if (coef == 1.0f) return;
+  for (int c = blockIdx.x; SCALE && c < 4 * nchunks; c += gridDim.x) {
+    const OptChunk ch = chunks[c >> 2];
+    const int from = (c & 3) * NORM_PART;
+    if (from >= ch.len) continue;
+    float* __restrict__ G = const_cast<float*>(rows[ch.row].g) + ch.start + from;
+    float4* __restrict__ G4 = reinterpret_cast<float4*>(G);
+    const int len = ch.len - from < NORM_PART ? ch.len - from : NORM_PART, len4 = len >> 2;
+    auto scaled = [&](float4 g) {
+      return make_float4(__fmul_rn(g.x, coef), __fmul_rn(g.y, coef), __fmul_rn(g.z, coef), __fmul_rn(g.w, coef));
+    };
+    int i = threadIdx.x;
+    for (; i + 3 * 256 < len4; i += 4 * 256) {
+      const float4 a = G4[i], b = G4[i + 256], c4 = G4[i + 512], d = G4[i + 768];
+      G4[i] = scaled(a);
+      G4[i + 256] = scaled(b);
+      G4[i + 512] = scaled(c4);
+      G4[i + 768] = scaled(d);
+    }
+    for (; i < len4; i += 256) G4[i] = scaled(G4[i]);
+    for (int k = (len4 << 2) + threadIdx.x; k < len; k += 256) G[k] = __fmul_rn(G[k], coef);
   }
 }
 
@@ -508,8 +544,9 @@ static int norm_code(float norm_type, float max_norm, const char* what) {
 
 template <int P>
 static void launch_norm(const Group& g, float max_norm, bool scale, float* out) {
-  const unsigned grid = opt_grid(g.nchunks);  // at most 4 CTAs per SM
-  const unsigned parts = grid < (unsigned)NORM_MAX_CTAS ? grid : (unsigned)NORM_MAX_CTAS;
+  TP_REQUIRE(g.nchunks <= INT_MAX / 8, "the gradients are too many for one norm");
+  const int most = sm_count() * 8 < NORM_MAX_CTAS ? sm_count() * 8 : NORM_MAX_CTAS, items = 4 * g.nchunks;
+  const unsigned parts = (unsigned)(items < 1 ? 1 : (items < most ? items : most)), grid = parts;
   TP_LAUNCH(k_grad_norm<P>, parts, 256, 0, g.rows, g.chunks, g.nchunks, g.partials);
   if (scale) TP_LAUNCH((k_grad_clip<P, true>), grid, 256, 0, g.rows, g.chunks, g.nchunks, g.partials, (int)parts,
                        max_norm, out);
