@@ -186,6 +186,33 @@ def test_many_rows(cuda_rt):
     check(cuda_rt, bf16(rng.standard_normal((1501, 2050)) * 3), rng.integers(0, 2050, 1501), 11, pad=1)
 
 
+@pytest.mark.parametrize("R", [4740, 9480, 20001])
+@pytest.mark.parametrize("V", [1, 2, 3, 10, 31, 64, 65, 127, 256, 264, 265, 400, 528, 529])
+def test_many_short_rows(cuda_rt, R, V):
+    """Rows enough for several to a warp: masks, equal logits, odd values."""
+    rng = np.random.default_rng(R + V)
+    x = bf16(rng.standard_normal((R, V)) * 2)
+    x[rng.random((R, V)) < 0.3] = -np.inf
+    x[::7] = 0.5
+    x[::11] = -np.inf
+    x[3::101, 0] = np.nan
+    x[4::103, V - 1] = np.inf
+    x[5::107] = LOW
+    x = np.concatenate([x[:400], x[-400:]])  # the oracle's rows
+    ids = rng.integers(-1, V, 800)
+    reps = (R + 799) // 800
+    big, K = np.tile(x, (reps, 1))[:R], min(V, 1 + V % 6 if R % 2 else 20)
+    got = forward(cuda_rt, big, np.tile(ids, reps)[:R], K, kind=R % 2, pad=V % 4)
+    want = logprobs(x, ids, K)
+    lp, ent = logprobs_tolerance(want, V)
+    tol = {"logp": lp(want["logp"]), "entropy": ent, "top_logp": lp(want["top_logp"])}
+    for r0 in range(0, R, 800):
+        n = min(800, R - r0)
+        assert np.array_equal(got["top_ids"][r0:r0 + n], want["top_ids"][:n])
+        for k in tol:
+            near(got[k][r0:r0 + n], want[k][:n], tol[k][:n], k)
+
+
 def test_outputs_left_out(cuda_rt):
     rt = cuda_rt
     x = np.random.default_rng(1).standard_normal((5, 3001)).astype(np.float32)

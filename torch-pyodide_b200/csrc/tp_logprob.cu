@@ -96,124 +96,124 @@ struct LpRow {
   }
 };
 
-// ---- short rows: a warp each, the row in registers ---------------------------------------
-// A warp takes `per` rows (at most 8) one after the other; lane r keeps row r's
-// statistics, so that logarithms and stores are done for all rows at once.  Lane l
-// holds the logits l + 32 k, k < N, of the row at hand and the best two of them.
-// The alternatives are found one by one: the warp's largest value, the lowest
-// index that has it; the lane it came from puts its second best in its place, or
-// looks for it when that is used up too.
-constexpr int LP_ROWS = 8;
-
-template <int N, bool TOP>
-__global__ void __launch_bounds__(256) k_logprobs_warp(const float* __restrict__ x, int64_t ld,
-                                                       const void* __restrict__ ids, int kind, int64_t R, int V,
-                                                       int per, int K, float* __restrict__ logp,
-                                                       float* __restrict__ entropy, float* __restrict__ stats,
-                                                       int32_t* __restrict__ top_ids, float* __restrict__ top_logp) {
+// ---- short rows: a group of L lanes each, the row in registers --------------------------
+// Lane l of the group holds the logits l + L k, k < N.  Smaller groups spend
+// fewer instructions per row on exchanging (a warp works on 32 / L rows at
+// once), larger ones finish a single row sooner.  The alternatives (K <= L of
+// them): at least K logits are as large as the K-th largest of the lanes' maxima;
+// what is that large is collected and the K best of it are ranked by counting.
+// Where more is equal than the list holds, they are found one after the other.
+template <int L, int N, bool TOP>
+__global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict__ x, int64_t ld,
+                                                        const void* __restrict__ ids, int kind, int64_t R, int V,
+                                                        int K, float* __restrict__ logp, float* __restrict__ entropy,
+                                                        float* __restrict__ stats, int32_t* __restrict__ top_ids,
+                                                        float* __restrict__ top_logp) {
   ::tp::pdl_enter();
-  __shared__ unsigned long long keys[8][TOP ? LP_ROWS * LP_MAX_TOP : 1];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t row0 = ((int64_t)blockIdx.x * 8 + w) * per;
-  if (row0 >= R) return;
-  const int rows = R - row0 < per ? (int)(R - row0) : per;
+  constexpr unsigned ALL = 0xffffffffu;
+  constexpr int G = 128 / L, CAND = 8 * L;
+  __shared__ unsigned long long cand[TOP ? G : 1][TOP ? CAND : 1];
+  __shared__ int cands[G];
+  const int l = threadIdx.x % L, g = threadIdx.x / L;
+  const int64_t row = (int64_t)blockIdx.x * G + g;
+  const bool live = row < R;  // lanes without a row only take part in the exchanges
+  const float* __restrict__ xr = x + row * ld;
   int t = -1;
-  if (logp && lane < rows) t = token_id(ids, kind, row0 + lane);
-  LpStat mine{-INFINITY, 0.0f, 0.0f};
-  for (int r = 0; r < rows; ++r) {
-    const float* __restrict__ xr = x + (row0 + r) * ld;
-    float v[N];
+  if (logp && live && l == 0) t = token_id(ids, kind, row);
+  float v[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int i = lane + 32 * k;
-      v[k] = i < V ? xr[i] : -INFINITY;
-    }
-    LpStat s{-INFINITY, 0.0f, 0.0f};
+  for (int k = 0; k < N; ++k) v[k] = live && l + L * k < V ? xr[l + L * k] : -INFINITY;
+  const float xt = t >= 0 && t < V ? xr[t] : 0.0f;
+  LpStat s{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < N; ++k) s.m = lp_max(s.m, v[k]);
-    for (int o = 16; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
+  for (int k = 0; k < N; ++k) s.m = lp_max(s.m, v[k]);
+  float tau = s.m;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s.add(v[k]);
-    for (int o = 16; o > 0; o >>= 1) {
-      s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
-      s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
-    }
-    if (lane == r) mine = s;
-    if (TOP) {
-      unsigned long long* out = keys[w] + r * K;
-      float b1 = -INFINITY, b2 = -INFINITY;
-      int i1 = 0, i2 = 0;
-      auto see = [&](float y, int k) {
-        if (y > b1) {
-          b2 = b1, i2 = i1;
-          b1 = y, i1 = k;
-        } else if (y > b2) {
-          b2 = y, i2 = k;
-        }
-      };
+  for (int o = L / 2; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(ALL, s.m, o));
 #pragma unroll
-      for (int k = 0; k < N; ++k) see(v[k], k);
-      bool second = true;
-      const bool odd = !(s.m < INFINITY);  // NaN or +inf in the row: no alternatives
-      for (int q = 0; q < K; ++q) {
-        const uint32_t o = odd || b1 == -INFINITY ? 0u : (uint32_t)(lp_key(b1, 0) >> 32);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, o);
-        const uint32_t i = o == top ? (uint32_t)(lane + 32 * i1) : UINT_MAX;
-        const uint32_t first = __reduce_min_sync(0xffffffffu, i);
-        if (lane == 0) out[q] = top ? (unsigned long long)top << 32 | (uint32_t)~first : 0ull;
-        if (top && i == first) {
-          if (second) {
-            b1 = b2, i1 = i2;
-            second = false;
-          } else {
-            const float y0 = b1;
-            const int k0 = i1;
-            b1 = b2 = -INFINITY;
+  for (int k = 0; k < N; ++k) s.add(v[k]);
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-              if (v[k] < y0 || (v[k] == y0 && k > k0)) see(v[k], k);
-            second = true;
-          }
-        }
+  for (int o = L / 2; o > 0; o >>= 1) {
+    s.S += __shfl_xor_sync(ALL, s.S, o);
+    s.T += __shfl_xor_sync(ALL, s.T, o);
+  }
+  const LpRow r(s);
+  if (live && l == 0) r.write(s, row, V, t, xt, logp, entropy, stats);
+  if constexpr (TOP) {
+#pragma unroll
+    for (int size = 2; size <= L; size <<= 1)  // the lanes' maxima in order, larger first
+#pragma unroll
+      for (int o = size >> 1; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(ALL, tau, o);
+        tau = ((l & o) == 0) == ((l & size) == 0 || size == L) ? fmaxf(tau, u) : fminf(tau, u);
       }
+    tau = fmaxf(__shfl_sync(ALL, tau, K - 1, L), -FLT_MAX);  // masked logits are no alternatives
+    unsigned long long some = 0ull;
+    if (!r.bad) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) some |= v[k] >= tau ? 1ull << k : 0ull;
     }
-  }
-  const LpRow a(mine);
-  if (lane < rows) {
-    const float xt = t >= 0 && t < V ? x[(row0 + lane) * ld + t] : 0.0f;
-    a.write(mine, row0 + lane, V, t, xt, logp, entropy, stats);
-  }
-  if (TOP) {
+    if (l == 0) cands[g] = 0;
     __syncwarp();
-    for (int e0 = 0; e0 < rows * K; e0 += 32) {
-      const int e = e0 + lane, r = e / K;
-      LpRow b = a;
-      b.bad = __shfl_sync(0xffffffffu, (int)a.bad, r & 31);
-      b.m = __shfl_sync(0xffffffffu, a.m, r & 31);
-      b.lnS = __shfl_sync(0xffffffffu, a.lnS, r & 31);
-      if (e < rows * K) b.write_top(keys[w][e], row0 * K + e, top_ids, top_logp);
+    while (some) {
+      const int k = __ffsll((long long)some) - 1;
+      some &= some - 1;
+      const int i = atomicAdd(&cands[g], 1);
+      if (i < CAND) cand[g][i] = lp_key(xr[l + L * k], (uint32_t)(l + L * k));
+    }
+    __syncwarp();
+    const int n = cands[g];
+    if (__any_sync(ALL, n > CAND)) {  // of any row of the warp
+      unsigned long long last = ~0ull;
+      for (int q = 0; q < K; ++q) {
+        unsigned long long best = 0ull;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const unsigned long long y = lp_key(v[k], (uint32_t)(l + L * k));
+          if (v[k] > -INFINITY && y < last && y > best) best = y;
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) {
+          const unsigned long long u = __shfl_xor_sync(ALL, best, o);
+          best = u > best ? u : best;
+        }
+        last = best;
+        if (live && l == 0) r.write_top(best, row * K + q, top_ids, top_logp);
+      }
+      return;
+    }
+    if (!live) return;
+    if (l >= n && l < K) r.write_top(0ull, row * K + l, top_ids, top_logp);
+    for (int i = l; i < n; i += L) {
+      const unsigned long long y = cand[g][i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += cand[g][j] > y;
+      if (above < K) r.write_top(y, row * K + above, top_ids, top_logp);
     }
   }
 }
 
-// ---- long rows: a CTA, or a cluster of CTAs, each ---------------------------------------
-// A CTA walks its part of the row once, 16 logits per thread at a time, with
-// running statistics per thread; the parts' statistics meet in the cluster's
-// first CTA over distributed shared memory, so one launch serves one row as well
-// as many and no workspace is shared between calls.
+// ---- longer rows: a team each -- a warp, a CTA or a cluster of CTAs ------------------------
+// A team walks its part of the row once, 16 logits per thread at a time, with
+// running statistics per thread.  Rows of a few thousand logits are a warp's: a
+// CTA's barriers would cost them as much as the walk.  Where there are few rows, a
+// cluster's CTAs take a part of one each; the parts' statistics meet in the
+// cluster's first CTA over distributed shared memory, so one launch serves one
+// row as well as many and no workspace is shared between calls.
 //
-// The alternatives cost the walk nothing: each thread only knows its maximum
-// and the batch it came from.  Call a thread's logits a unit, and its best (value,
-// then lower index) the unit's key.  Whatever the K best logits of the part are,
-// each is at least as good as the K-th best unit key, so they all stand in the
-// K units with the best keys: these are read again (from L2: K / 256 of the
-// part), what is at least as good as the K-th key is collected, and the K best of
-// that are ranked by counting.
-constexpr int LP_NT = 256;
-constexpr int LP_CAND = 512;
+// The alternatives cost the walk next to nothing: each thread knows the maxima
+// of its four vectors (over all batches): four units.  With tau a value that at
+// least K units reach, the K best logits all stand in units that reach it: these
+// are read again (from L2: one to four times K of the team's 4 NT), what reaches
+// tau is collected, and the K best of it are ranked by counting.  Where so many
+// logits are equal that the units or the collected logits do not fit their
+// lists, whole threads are told apart by the index of their maximum too, which
+// leaves exactly K of them.
 
 // A part of a row as 16-byte vectors: vector j holds the logits 4 j - a ..
 // 4 j - a + 3 of the part, a = how far the part starts past a 16-byte boundary.
+// Batch b of thread t: the vectors 4 NT b + NT q + t, q < 4.
+template <int NT>
 struct LpPart {
   const float* base;  // the boundary at or below the part's first logit
   int a, end;         // its logits are base[a .. end)
@@ -225,6 +225,7 @@ struct LpPart {
     end = a + (int)(hi > lo_ ? hi - lo_ : 0);
     lo = lo_ - a;
   }
+  __device__ __forceinline__ int batches() const { return (end + 16 * NT - 1) / (16 * NT); }
   __device__ __forceinline__ float4 edge(int j) const {
     const int u = 4 * j;
     float4 v;
@@ -237,57 +238,64 @@ struct LpPart {
   __device__ __forceinline__ float4 vec(int j) const {
     return 4 * j >= a && 4 * j + 4 <= end ? *reinterpret_cast<const float4*>(base + 4 * j) : edge(j);
   }
-  // the 4 vectors of thread t in batch b
   __device__ __forceinline__ void batch(int b, int t, float4 (&v)[4]) const {
-    const int j = b * 4 * LP_NT + t;
-    if ((b > 0 || a == 0) && 4 * (b + 1) * 4 * LP_NT <= end) {
+    const int j = b * 4 * NT + t;
+    if ((b > 0 || a == 0) && 16 * NT * (b + 1) <= end) {
       const float4* p = reinterpret_cast<const float4*>(base) + j;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = p[q * LP_NT];
+      for (int q = 0; q < 4; ++q) v[q] = p[q * NT];
     } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = vec(j + q * LP_NT);
+      for (int q = 0; q < 4; ++q) v[q] = vec(j + q * NT);
     }
   }
 };
 
+template <int NT>
 struct LpShared {
-  float f[8];
-  LpStat part;                          // read by the cluster's first CTA
-  unsigned long long top[LP_MAX_TOP];   // the part's alternatives, likewise
-  unsigned long long unit[LP_NT];       // keys of the better units
-  unsigned char owner[LP_NT];           // and their threads
-  unsigned char chosen[LP_MAX_TOP];     // the threads of the K best
-  unsigned long long cand[LP_CAND];
-  unsigned long long k[8], least;
+  static constexpr int CAND = NT == 32 ? 256 : 512;  // collected logits
+  static constexpr int LIST = NT == 32 ? 128 : 256;  // units read again
+  LpStat warp[NT / 32], part;          // part: read by the cluster's first CTA
+  float kth[NT / 32];                  // per warp: a value that K / (NT / 32) of its threads' maxima reach
+  unsigned long long top[LP_MAX_TOP];  // the part's alternatives, read by the first CTA too
+  unsigned short chosen[LIST];         // the units read again: 4 thread + vector
+  float value[LIST], tau;              // and their maxima; the K-th largest of these
+  unsigned short owner[NT];            // ties: threads
+  unsigned long long cand[CAND];
+  unsigned long long k[NT / 32], least;
   int units, cands;
 };
 
-__device__ __forceinline__ float lp_block_max(float v, float* sh) {
-  for (int o = 16; o > 0; o >>= 1) v = lp_max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
-#pragma unroll
-  for (int w = 1; w < LP_NT / 32; ++w) v = lp_max(v, sh[w]);
-  __syncthreads();
-  return v;
+template <int NT>
+__device__ __forceinline__ void lp_sync() {
+  if (NT == 32) __syncwarp();
+  else __syncthreads();
 }
-__device__ __forceinline__ float lp_block_sum(float v, float* sh) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh[0];
+
+// the warp's largest value; a NaN in any lane is kept
+__device__ __forceinline__ float lp_warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// the warp's values in order, larger first
+__device__ __forceinline__ float lp_sorted(float v, int lane) {
 #pragma unroll
-  for (int w = 1; w < LP_NT / 32; ++w) v += sh[w];
-  __syncthreads();
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, v, o);
+      v = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(v, u) : fminf(v, u);
+    }
   return v;
 }
 
 // keys[0..n) into out[0..K) in order of rank (0 where there are fewer); keys differ
-__device__ __forceinline__ void lp_rank(const unsigned long long* keys, int n, int K, unsigned long long* out) {
-  if (threadIdx.x >= n && threadIdx.x < K) out[threadIdx.x] = 0ull;
-  for (int i = threadIdx.x; i < n; i += LP_NT) {
+template <int NT>
+__device__ __forceinline__ void lp_rank(int t, const unsigned long long* keys, int n, int K, unsigned long long* out) {
+  if (t >= n && t < K) out[t] = 0ull;
+  for (int i = t; i < n; i += NT) {
     const unsigned long long k = keys[i];
     int r = 0;
     for (int j = 0; j < n; ++j) r += keys[j] > k;
@@ -295,98 +303,165 @@ __device__ __forceinline__ void lp_rank(const unsigned long long* keys, int n, i
   }
 }
 
-// The K best keys of the part into sh.top.  m: this thread's maximum, mb: its batch.
-__device__ void lp_select(const LpPart& p, float m, int mb, int K, LpShared& sh) {
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  // A value that at least K units reach: the least over the warps of each warp's
-  // ceil(K / 8)-th largest maximum.
-  float v = m;
-  for (int size = 2; size <= 32; size <<= 1)
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffffu, v, o);
-      const bool down = (lane & size) == 0 || size == 32;  // larger values first
-      v = ((lane & o) == 0) == down ? fmaxf(v, u) : fminf(v, u);
-    }
-  const int kq = (K + LP_NT / 32 - 1) / (LP_NT / 32);
-  if (lane == kq - 1) sh.f[w] = v;
-  if (t == 0) sh.units = sh.cands = 0;
-  __syncthreads();
-  float tau = sh.f[0];
+// Shows `take` every logit of the units chosen[0..n), by all threads of the team.
+template <int NT, class F>
+__device__ __forceinline__ void lp_reread(int t, const LpPart<NT>& p, const unsigned short* chosen, int n, F take) {
+  const int nv = (p.end + 3) >> 2, per = p.batches();
+  const float inv = 1.0f / (float)per;  // (i + 0.5) / per is at least 0.5 / per off a whole number; i < 2^20
+  for (int i0 = t; i0 < n * per; i0 += 2 * NT) {
+    float4 q[2];
+    int j[2];
 #pragma unroll
-  for (int i = 1; i < LP_NT / 32; ++i) tau = fminf(tau, sh.f[i]);
-  if (m >= tau && m > -INFINITY) {  // where in its batch this unit's best stands
+    for (int c = 0; c < 2; ++c) {
+      const int i = i0 + c * NT, s = (int)(((float)i + 0.5f) * inv);
+      j[c] = nv;
+      if (i < n * per) {
+        const int code = chosen[s];
+        j[c] = 4 * NT * (i - s * per) + NT * (code & 3) + (code >> 2);
+      }
+      if (j[c] < nv) q[c] = p.vec(j[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (j[c] < nv) {
+        const uint32_t at = (uint32_t)(p.lo + 4 * j[c]);
+        take(q[c].x, at);
+        take(q[c].y, at + 1);
+        take(q[c].z, at + 2);
+        take(q[c].w, at + 3);
+      }
+  }
+}
+
+// The K best keys of the part into sh.top, by thread t of the team.  um: this
+// thread's unit maxima, mb: the batch its largest came from first, tau: a value
+// that at least K units reach; the counters are 0.
+template <int NT>
+__device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int mb, float tau, int K,
+                          LpShared<NT>& sh) {
+  tau = fmaxf(tau, -FLT_MAX);  // masked logits are no alternatives
+  unsigned mine = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) mine |= um[q] >= tau ? 1u << q : 0u;
+  const bool in = mine != 0u;
+  while (mine) {
+    const int q = __ffs(mine) - 1, i = atomicAdd(&sh.units, 1);
+    mine &= mine - 1;
+    if (i < LpShared<NT>::LIST) {
+      sh.chosen[i] = (unsigned short)(4 * t + q);
+      sh.value[i] = q == 0 ? um[0] : (q == 1 ? um[1] : (q == 2 ? um[2] : um[3]));
+    }
+  }
+  lp_sync<NT>();
+  int n = sh.units;
+  if (n <= LpShared<NT>::LIST && n > K && n * p.batches() > 2 * NT) {
+    // much to read: first the K-th largest of them, and only what reaches that
+    constexpr int PER = LpShared<NT>::LIST / NT;
+    unsigned short code[PER];
+    bool keep[PER];
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      const int u = t + c * NT;
+      keep[c] = false;
+      if (u < n) {
+        const float y = sh.value[u];
+        int above = 0, same = 0;
+        for (int j = 0; j < n; ++j) {
+          above += sh.value[j] > y;
+          same += sh.value[j] == y;
+        }
+        code[c] = sh.chosen[u];
+        keep[c] = above < K;
+        if (keep[c] && above + same >= K) sh.tau = y;
+      }
+    }
+    lp_sync<NT>();
+    if (t == 0) sh.units = 0;
+    lp_sync<NT>();
+    tau = sh.tau;
+#pragma unroll
+    for (int c = 0; c < PER; ++c)
+      if (keep[c]) sh.chosen[atomicAdd(&sh.units, 1)] = code[c];
+    lp_sync<NT>();
+    n = sh.units;
+  }
+  auto add = [&](float x, uint32_t at) {
+    const int i = atomicAdd(&sh.cands, 1);
+    if (i < LpShared<NT>::CAND) sh.cand[i] = lp_key(x, at);
+  };
+  if (n <= LpShared<NT>::LIST) {
+    lp_reread<NT>(t, p, sh.chosen, n, [&](float x, uint32_t at) {
+      if (x >= tau) add(x, at);
+    });
+    lp_sync<NT>();
+    const int nc = sh.cands;
+    if (nc <= LpShared<NT>::CAND) {
+      lp_rank<NT>(t, sh.cand, nc, K, sh.top);
+      return;
+    }
+  }
+  // Ties: threads in the place of units, and where in its batch the maximum of each stands.
+  lp_sync<NT>();
+  if (t == 0) sh.units = sh.cands = 0, sh.least = 0ull;
+  lp_sync<NT>();
+  if (in) {
+    const float m = fmaxf(fmaxf(um[0], um[1]), fmaxf(um[2], um[3]));
     float4 x[4];
     p.batch(mb, t, x);
     int at = 0;
 #pragma unroll
     for (int q = 3; q >= 0; --q) {
-      const int u = 4 * (mb * 4 * LP_NT + q * LP_NT + t);
+      const int u = 4 * (mb * 4 * NT + q * NT + t);
       if (x[q].w == m) at = u + 3;
       if (x[q].z == m) at = u + 2;
       if (x[q].y == m) at = u + 1;
       if (x[q].x == m) at = u;
     }
     const int i = atomicAdd(&sh.units, 1);
-    sh.unit[i] = lp_key(m, (uint32_t)(p.lo + at));
-    sh.owner[i] = (unsigned char)t;
+    sh.cand[i] = lp_key(m, (uint32_t)(p.lo + at));
+    sh.owner[i] = (unsigned short)t;
   }
-  __syncthreads();
-  const int n = sh.units, chosen = n < K ? n : K;
-  if (t == 0 && n < K) sh.least = 0ull;
-  if (t < n) {
-    const unsigned long long k = sh.unit[t];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += sh.unit[j] > k;
-    if (r < K) sh.chosen[r] = sh.owner[t];
-    if (r == K - 1) sh.least = k;
+  lp_sync<NT>();
+  n = sh.units;
+  const int chosen = 4 * (n < K ? n : K);
+  for (int u = t; u < n; u += NT) {
+    const unsigned long long k = sh.cand[u];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
+    if (above < K)
+      for (int q = 0; q < 4; ++q) sh.chosen[4 * above + q] = (unsigned short)(4 * sh.owner[u] + q);
+    if (above == K - 1) sh.least = k;
   }
-  __syncthreads();
+  lp_sync<NT>();
   const unsigned long long least = sh.least;
-  const int nv = (p.end + 3) >> 2;
-  for (int s = w; s < chosen; s += LP_NT / 32)
-    for (int j = sh.chosen[s] + LP_NT * lane; j < nv; j += LP_NT * 32) {
-      const float4 q = p.vec(j);
-      const float e[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const unsigned long long k = lp_key(e[c], (uint32_t)(p.lo + 4 * j + c));
-        if (e[c] > -INFINITY && k >= least) {
-          const int i = atomicAdd(&sh.cands, 1);
-          if (i < LP_CAND) sh.cand[i] = k;
-        }
-      }
-    }
-  __syncthreads();
+  lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
+    if (x > -INFINITY && lp_key(x, at) >= least) add(x, at);
+  });
+  lp_sync<NT>();
   const int nc = sh.cands;
-  if (nc <= LP_CAND) {
-    lp_rank(sh.cand, nc, K, sh.top);
+  if (nc <= LpShared<NT>::CAND) {
+    lp_rank<NT>(t, sh.cand, nc, K, sh.top);
     return;
   }
-  // More than the list holds (a few units with most of the row's large values):
+  // More than the list holds (a few threads with most of the row's large values):
   // one alternative after the other, the best that is worse than the one before.
   unsigned long long last = ~0ull;
   for (int q = 0; q < K; ++q) {
     unsigned long long best = 0ull;
-    for (int s = w; s < chosen; s += LP_NT / 32)
-      for (int j = sh.chosen[s] + LP_NT * lane; j < nv; j += LP_NT * 32) {
-        const float4 x = p.vec(j);
-        const float e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const unsigned long long k = lp_key(e[c], (uint32_t)(p.lo + 4 * j + c));
-          if (e[c] > -INFINITY && k < last && k > best) best = k;
-        }
-      }
+    lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
+      const unsigned long long k = lp_key(x, at);
+      if (x > -INFINITY && k < last && k > best) best = k;
+    });
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
       best = u > best ? u : best;
     }
-    if (lane == 0) sh.k[w] = best;
-    __syncthreads();
-    for (int i = 0; i < LP_NT / 32; ++i) best = sh.k[i] > best ? sh.k[i] : best;
+    if ((t & 31) == 0) sh.k[t >> 5] = best;
+    lp_sync<NT>();
+    for (int i = 0; i < NT / 32; ++i) best = sh.k[i] > best ? sh.k[i] : best;
     if (t == 0) sh.top[q] = best;
     last = best;
-    __syncthreads();
+    lp_sync<NT>();
   }
 }
 
@@ -409,18 +484,27 @@ __device__ __forceinline__ unsigned long long lp_peer_u64(uint32_t at) {
   return v;
 }
 
-// parts: CTAs per row, the cluster's size
-template <bool TOP>
-__global__ void __launch_bounds__(LP_NT) k_logprobs_long(const float* __restrict__ x, int64_t ld,
-                                                         const void* __restrict__ ids, int kind, int64_t V, int parts,
-                                                         int K, float* __restrict__ logp, float* __restrict__ entropy,
-                                                         float* __restrict__ stats, int32_t* __restrict__ top_ids,
-                                                         float* __restrict__ top_logp) {
+// NT: threads of a team (a warp: four teams to a CTA); parts: CTAs per row, the
+// cluster's size
+template <int NT, bool TOP>
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT)
+    k_logprobs_long(const float* __restrict__ x, int64_t ld, const void* __restrict__ ids, int kind, int64_t R,
+                    int64_t V, int parts, int K, float* __restrict__ logp, float* __restrict__ entropy,
+                    float* __restrict__ stats, int32_t* __restrict__ top_ids, float* __restrict__ top_logp) {
   ::tp::pdl_enter();
-  __shared__ LpShared sh;
-  const int t = threadIdx.x;
-  const int64_t row = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x - row * parts);
+  constexpr int TEAMS = NT == 32 ? 4 : 1, WARPS = NT / 32;
+  __shared__ LpShared<NT> shared[TEAMS];
+  LpShared<NT>& sh = shared[threadIdx.x / NT];
+  const int t = threadIdx.x % NT, lane = t & 31;
+  int64_t row;
+  int part = 0;
+  if (NT == 32) {
+    row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / NT;
+    if (row >= R) return;
+  } else {
+    row = blockIdx.x / parts;
+    part = (int)(blockIdx.x - row * parts);
+  }
   const float* __restrict__ xr = x + row * ld;
   int tok = -1;
   float xt = 0.0f;
@@ -430,20 +514,24 @@ __global__ void __launch_bounds__(LP_NT) k_logprobs_long(const float* __restrict
   }
   const int64_t per = (V + parts - 1) / parts;
   const int64_t lo = per * part < V ? per * part : V, hi = lo + per < V ? lo + per : V;
-  const LpPart p(xr, lo, hi);
-  const int batches = (p.end + 16 * LP_NT - 1) / (16 * LP_NT);
+  const LpPart<NT> p(xr, lo, hi);
+  const int batches = p.batches();
   LpStat s{-INFINITY, 0.0f, 0.0f};
+  float um[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   int mb = 0;
-  float4 next[4];
-  p.batch(0, t, next);
   for (int b = 0; b < batches; ++b) {
     float4 v[4];
+    p.batch(b, t, v);
+    float m;
+    if (TOP) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = next[q];
-    if (b + 1 < batches) p.batch(b + 1, t, next);
-    float m = s.m;
+      for (int q = 0; q < 4; ++q) um[q] = lp_max(um[q], lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
+      m = lp_max(lp_max(um[0], um[1]), lp_max(um[2], um[3]));
+    } else {
+      m = s.m;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) m = lp_max(m, lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
+      for (int q = 0; q < 4; ++q) m = lp_max(m, lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
+    }
     if (m != s.m) {
       s.move(m);
       mb = b;
@@ -456,15 +544,61 @@ __global__ void __launch_bounds__(LP_NT) k_logprobs_long(const float* __restrict
       s.add(v[q].w);
     }
   }
-  const float own = s.m;
-  s.move(lp_block_max(own, sh.f));
-  s.S = lp_block_sum(s.S, sh.f);
-  s.T = lp_block_sum(s.T, sh.f);
-  if (TOP) {
-    if (s.m < INFINITY) lp_select(p, own, mb, K, sh);  // not with a NaN or +inf in the part
-    __syncthreads();
+  float own = s.m;
+  const float most = lp_warp_max(own);
+  s.move(most);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s.S += __shfl_xor_sync(0xffffffffu, s.S, o);
+    s.T += __shfl_xor_sync(0xffffffffu, s.T, o);
   }
-  if (parts > 1) {
+  float tau = most;
+  if (TOP) {  // the ceil(K / WARPS)-th largest of the threads' maxima, equal ones counted once
+    const int kq = (K + WARPS - 1) / WARPS;
+    if (kq <= 5) {
+      for (int i = 1; i < kq; ++i) {
+        if (own == tau) own = -INFINITY;
+        tau = lp_warp_max(own);
+      }
+    } else {
+      tau = lp_sorted(own, lane);
+      tau = __shfl_sync(0xffffffffu, tau, kq - 1);
+    }
+    if (t == 0) sh.units = sh.cands = 0, sh.least = 0ull;
+  }
+  if (WARPS > 1) {
+    if (lane == 0) {
+      sh.warp[t >> 5] = s;
+      sh.kth[t >> 5] = tau;
+    }
+    __syncthreads();
+    s = sh.warp[0];
+    float m = s.m;
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) m = lp_max(m, sh.warp[i].m);
+    if (t < 32) {  // the sums are the first warp's business
+      s.move(m);
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) {
+        LpStat o = sh.warp[i];
+        o.move(m);
+        s.S += o.S;
+        s.T += o.T;
+      }
+    }
+    s.m = m;
+    if (TOP) {
+      tau = sh.kth[0];
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) tau = fminf(tau, sh.kth[i]);
+    }
+  }
+  if (TOP) {
+    if (WARPS == 1) __syncwarp();
+    if (s.m < INFINITY) lp_select<NT>(t, p, um, mb, tau, K, sh);  // not with a NaN or +inf in the part
+    lp_sync<NT>();
+  }
+  if (NT != 32 && parts > 1) {
     if (t == 0) sh.part = s;
     lp_cluster_sync();
     if (part == 0) {
@@ -483,14 +617,14 @@ __global__ void __launch_bounds__(LP_NT) k_logprobs_long(const float* __restrict
       if (TOP && m < INFINITY) {
         // the parts' lists (0-padded) side by side, then the best of them
         const int n = parts * K;
-        for (int i = t; i < n; i += LP_NT) {
+        for (int i = t; i < n; i += NT) {
           const int c = i / K;
           sh.cand[i] = lp_peer_u64(lp_peer(&sh.top[i - c * K], c));
         }
         __syncthreads();
         if (t < K) sh.top[t] = 0ull;
         __syncthreads();
-        for (int i = t; i < n; i += LP_NT) {
+        for (int i = t; i < n; i += NT) {
           const unsigned long long k = sh.cand[i];
           int r = 0;
           for (int j = 0; j < n; ++j) r += sh.cand[j] > k;
@@ -502,6 +636,7 @@ __global__ void __launch_bounds__(LP_NT) k_logprobs_long(const float* __restrict
     lp_cluster_sync();
     if (part != 0) return;
   }
+  if (t >= 32) return;
   const LpRow r(s);
   if (t == 0) r.write(s, row, V, tok, xt, logp, entropy, stats);
   if (TOP && t < K) r.write_top(r.bad || r.none ? 0ull : sh.top[t], row * K + t, top_ids, top_logp);
@@ -612,36 +747,29 @@ __global__ void __launch_bounds__(256) k_logprobs_bwd(const float* x, int64_t ld
   }
 }
 
-// Rows up to this long are a warp's.
-constexpr int64_t LP_WARP_MAX = 1024;
+// Rows up to this long are held in registers.
+constexpr int64_t LP_SHORT = 1024;
 
-template <bool TOP>
-static void launch_logprobs_warp(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int V, int K,
-                                 float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp) {
-  // one row per warp until there are warps for every scheduler several times over
-  int per = 1;
-  while (per < LP_ROWS && R >= (int64_t)sm_count() * 64 * 2 * per) per *= 2;
-  const unsigned grid = (unsigned)((R + 8 * per - 1) / (8 * per));
-#define TP_LP_WARP(N)                                                                                                 \
-  if (V <= 32 * N) {                                                                                                  \
-    TP_LAUNCH((k_logprobs_warp<N, TOP>), grid, 256, 0, x, ld, ids, kind, R, V, per, K, logp, entropy, stats, top_ids, \
-              top_logp);                                                                                              \
-    return;                                                                                                           \
+template <int L, bool TOP>
+static void launch_logprobs_short(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int V, int K,
+                                  float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp) {
+  const unsigned grid = (unsigned)((R + 128 / L - 1) / (128 / L));
+#define TP_LP_SHORT(N)                                                                                             \
+  if (V <= L * N) {                                                                                                \
+    TP_LAUNCH((k_logprobs_short<L, N, TOP>), grid, 128, 0, x, ld, ids, kind, R, V, K, logp, entropy, stats, top_ids, \
+              top_logp);                                                                                           \
+    return;                                                                                                        \
   }
-  TP_LP_WARP(1)
-  TP_LP_WARP(2)
-  TP_LP_WARP(3)
-  TP_LP_WARP(4)
-  TP_LP_WARP(6)
-  TP_LP_WARP(8)
-  TP_LP_WARP(9)
-  TP_LP_WARP(12)
-  TP_LP_WARP(16)
-  TP_LP_WARP(20)
-  TP_LP_WARP(24)
-  TP_LP_WARP(28)
-  TP_LP_WARP(32)
-#undef TP_LP_WARP
+  TP_LP_SHORT(2)
+  TP_LP_SHORT(4)
+  TP_LP_SHORT(8)
+  TP_LP_SHORT(12)
+  TP_LP_SHORT(16)
+  TP_LP_SHORT(20)
+  TP_LP_SHORT(24)
+  TP_LP_SHORT(28)
+  TP_LP_SHORT(33)
+#undef TP_LP_SHORT
 }
 
 // As TP_LAUNCH, in clusters of `cluster` CTAs.
@@ -663,32 +791,68 @@ static void launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned blo
   g_launches++;
 }
 
+// Threads of a row's team.  Times with 5 alternatives, in us, 512 MB of logits:
+//
+//            4096   8192  16384  50021 logits a row      1999 rows of 50021   64 rows of 4096
+//   warp       97     98    108    120                                  100               9.4
+//   128       153    112     99     98                                   70               5.4
+//   256       178    117     97     96                                   74               6.6
+//
+// A warp's row has no barrier, and its walk is long only if rows are few; 128
+// threads leave the last rows of a few hundred per SM wave less alone than 256.
+static int lp_threads(int64_t R, int64_t V) {
+  const int64_t sms = sm_count();
+  if (V <= 8192 && R >= 16 * sms) return 32;
+  if (V <= 4096) return 128;
+  return R >= 6 * sms && R < 16 * sms ? 128 : 256;
+}
+
 void launch_logprobs(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int64_t V, int K, float* logp,
                      float* entropy, float* stats, int32_t* top_ids, float* top_logp) {
   if (R == 0) return;
-  if (V <= LP_WARP_MAX) {
-    if (K) launch_logprobs_warp<true>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);
-    else launch_logprobs_warp<false>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);
+  if (V <= LP_SHORT) {
+    // the smallest group whose lanes hold the row and whose warps still fill the SMs
+    const int64_t warps = (int64_t)sm_count() * 16;
+    const int L = V <= 8 * 33 && K <= 8 && R >= 4 * warps ? 8 : (V <= 16 * 33 && K <= 16 && R >= 2 * warps ? 16 : 32);
+#define TP_LP_GROUP(L)                                                                                                \
+  if (K) launch_logprobs_short<L, true>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);   \
+  else launch_logprobs_short<L, false>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);
+    if (L == 8) {
+      TP_LP_GROUP(8)
+    } else if (L == 16) {
+      TP_LP_GROUP(16)
+    } else {
+      TP_LP_GROUP(32)
+    }
+#undef TP_LP_GROUP
     return;
   }
+  const int nt = lp_threads(R, V);
   // more CTAs per row while the rows alone leave SMs empty and a part keeps a batch
   int parts = 1;
-  while (parts < 8 && R * parts < 4 * (int64_t)sm_count() && V / (2 * parts) >= 2048) parts *= 2;
-  TP_REQUIRE(R * parts <= INT_MAX, "token_logprobs: %lld rows are too many", (long long)R);
-  const unsigned grid = (unsigned)(R * parts);
-  if (K)
-    launch_cluster(k_logprobs_long<true>, grid, LP_NT, parts, x, ld, ids, kind, V, parts, K, logp, entropy, stats,
-                   top_ids, top_logp);
-  else
-    launch_cluster(k_logprobs_long<false>, grid, LP_NT, parts, x, ld, ids, kind, V, parts, K, logp, entropy, stats,
-                   top_ids, top_logp);
+  while (nt == 256 && parts < 8 && R * parts < 4 * (int64_t)sm_count() && V / (2 * parts) >= 2048) parts *= 2;
+  const int64_t ctas = nt == 32 ? (R + 3) / 4 : R * parts;
+  TP_REQUIRE(ctas <= INT_MAX, "token_logprobs: %lld rows are too many", (long long)R);
+#define TP_LP_LONG(NT)                                                                                                 \
+  if (nt == NT) {                                                                                                      \
+    if (K)                                                                                                             \
+      launch_cluster(k_logprobs_long<NT, true>, (unsigned)ctas, NT == 32 ? 128 : NT, parts, x, ld, ids, kind, R, V, parts, \
+                     K, logp, entropy, stats, top_ids, top_logp);                                                      \
+    else                                                                                                               \
+      launch_cluster(k_logprobs_long<NT, false>, (unsigned)ctas, NT == 32 ? 128 : NT, parts, x, ld, ids, kind, R, V, parts, \
+                     K, logp, entropy, stats, top_ids, top_logp);                                                      \
+  }
+  TP_LP_LONG(32)
+  TP_LP_LONG(128)
+  TP_LP_LONG(256)
+#undef TP_LP_LONG
 }
 
 void launch_logprobs_bwd(const float* x, int64_t ld, const void* ids, int kind, const float* stats,
                          const float* entropy, const float* dlogp, const float* dentropy, int64_t R, int64_t V,
                          float* dx, int64_t ldd) {
   if (R == 0) return;
-  if (V <= LP_WARP_MAX) {
+  if (V <= LP_SHORT) {
     TP_LAUNCH(k_logprobs_bwd_warp, (unsigned)((R + 7) / 8), 256, 0, x, ld, ids, kind, stats, entropy, dlogp, dentropy,
               R, (int)V, dx, ldd);
     return;
