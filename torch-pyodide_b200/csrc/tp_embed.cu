@@ -10,7 +10,6 @@
 #include <climits>
 
 #include "tp_core.h"
-#include "tp_fastdiv.cuh"
 #include "tp_launch.h"
 #include "tp_token.cuh"
 
@@ -76,42 +75,55 @@ __global__ void __launch_bounds__(EMB_NT) k_embed(const float* __restrict__ tabl
   }
 }
 
-// ---- gradient of a few tokens ---------------------------------------------------------
-// One CTA per (position, 256 columns): the first position of a token sums all
-// of them, in order.  Reads the ids n times over, which for few is less than
-// sorting them costs.
-__global__ void __launch_bounds__(256) k_embed_bwd_few(const float* __restrict__ dout, int64_t ldo,
-                                                       const void* __restrict__ ids, int kind, int n, int64_t V,
-                                                       int64_t D, int chunks, float scale, int64_t pad,
-                                                       float* __restrict__ dtable, int64_t ld) {
+// ---- gradient of a few tokens, added to an existing one -----------------------------------
+// One CTA per (position, 256 columns), which compares its token with all ids at
+// once: the first position of a token sums all of them, in order.  Reads the ids
+// n times over, and a frequent token's rows one after the other: 256 x 1024 takes
+// 5.7 us against 14.1 sorted, 1024 x 4096 23.6 against 22.5.
+constexpr int EMB_FEW = 512;
+
+template <int VEC>
+__global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dout, int64_t ldo,
+                                                   const void* __restrict__ ids, int kind, int n, int64_t V,
+                                                   int64_t cols, int chunks, float scale, int64_t pad,
+                                                   float* __restrict__ dtable, int64_t ld) {
   ::tp::pdl_enter();
-  __shared__ uint32_t hit[8];
+  __shared__ uint32_t hits[EMB_FEW / 32];
+  const int t = threadIdx.x, lane = t & 31;
   const int i = blockIdx.x / chunks;
-  const int64_t d = (int64_t)(blockIdx.x - i * chunks) * 256 + threadIdx.x;
-  const int64_t v = token_id(ids, kind, i);
+  const int64_t c = (int64_t)(blockIdx.x - i * chunks) * 256 + t;
+  const int v = token_id(ids, kind, i);
+  int u[EMB_FEW / 256];
+#pragma unroll
+  for (int r = 0; r < EMB_FEW / 256; ++r) u[r] = r * 256 + t < n ? token_id(ids, kind, r * 256 + t) : -1;
   if (v < 0 || v >= V || v == pad) return;
   bool earlier = false;
-  for (int j = threadIdx.x; j < i; j += 256) earlier |= token_id(ids, kind, j) == v;
-  if (__syncthreads_or(earlier)) return;
-  float acc = 0.0f;
-  for (int j0 = i; j0 < n; j0 += 256) {
-    const int j = j0 + threadIdx.x;
-    const uint32_t b = __ballot_sync(0xffffffffu, j < n && token_id(ids, kind, j) == v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) hit[threadIdx.x >> 5] = b;
-    __syncthreads();
-    float part = 0.0f;  // chains of at most 256 additions, then of n / 256
-    for (int w = 0; w < 8; ++w)
-      for (uint32_t q = hit[w]; q; q &= q - 1)
-        if (d < D) part += dout[(int64_t)(j0 + 32 * w + __ffs(q) - 1) * ldo + d];
-    acc += part;
+#pragma unroll
+  for (int r = 0; r < EMB_FEW / 256; ++r) {
+    earlier |= u[r] == v && r * 256 + t < i;
+    const uint32_t b = __ballot_sync(0xffffffffu, u[r] == v);
+    if (lane == 0) hits[r * 8 + (t >> 5)] = b;
   }
-  if (d < D) dtable[v * ld + d] += acc * scale;
+  if (__syncthreads_or(earlier)) return;
+  if (c >= cols) return;
+  const Col<VEC> old = Col<VEC>::load(dtable + (int64_t)v * ld, c);
+  Col<VEC> acc = Col<VEC>::zero();
+  for (int w0 = i >> 8 << 3; 32 * w0 < n; w0 += 8) {  // chains of at most 256 additions, then of n / 256
+    Col<VEC> part = Col<VEC>::zero();
+#pragma unroll
+    for (int w = w0; w < w0 + 8; ++w)
+      for (uint32_t q = hits[w]; q; q &= q - 1)
+        part.add(Col<VEC>::load(dout + (int64_t)(32 * w + __ffs(q) - 1) * ldo, c));
+    acc.add(part);
+  }
+  Col<VEC> r = acc.times(scale);
+  r.add(old);
+  r.store(dtable + (int64_t)v * ld, c);
 }
 
 // ---- gradient of many tokens: positions sorted by token, then summed -----------------------
-// Sorting is one launch of CTAs that share nothing.  Token v belongs to CTA
-// v mod G, as its token v / G (neighbouring ids, of like frequency, go to
+// Sorting is one launch of G = 2^g CTAs that share nothing.  Token v belongs to
+// CTA v mod G, as its token v / G (neighbouring ids, of like frequency, go to
 // different CTAs).  Each CTA reads all ids: it counts those of the CTAs before
 // it, which is where its own begin, and the tokens of its own per warp; after a
 // scan over (token, warp) the warps place their positions in order.  A position
@@ -121,33 +133,34 @@ __global__ void __launch_bounds__(256) k_embed_bwd_few(const float* __restrict__
 constexpr int SORT_NT = 1024;
 constexpr int SORT_WARPS = SORT_NT / 32;
 constexpr int SORT_TOKENS = 512;          // tokens of one CTA, at most
-constexpr int SORT_WORDS = 32768;         // positions / 32 whose hits are kept in shared memory
+constexpr int SORT_WORDS = 16384;         // positions / 32 whose hits are kept in shared memory
 constexpr int SORT_U = 16;                // ids of a thread in flight
 
 struct EmbedSort {
-  FastDiv ctas;   // G
+  int g;          // log2 of the CTAs
   int per;        // tokens of one CTA, W
   int64_t n;
-  int V, pad, kind;
+  int V, pad;
   const void* ids;
   int32_t* start;  // [G W + 1]: where the run of key owner * W + local starts; the last: how many positions there are
   int32_t* pos;    // [n]
   int32_t* tok;    // [n]
-  __device__ __forceinline__ bool valid(int v) const { return v >= 0 && v < V && v != pad; }
-  __device__ __forceinline__ int key(int v) const {
-    const int q = (int)ctas.div((uint32_t)v);
-    return (v - q * (int)ctas.d) * per + q;
-  }
-  __device__ __forceinline__ int total() const { return start[(int64_t)ctas.d * per]; }
+  __device__ __forceinline__ bool valid(int v) const { return (uint32_t)v < (uint32_t)V && v != pad; }
+  __device__ __forceinline__ int owner(int v) const { return v & ((1 << g) - 1); }
+  __device__ __forceinline__ int local(int v) const { return v >> g; }
+  __device__ __forceinline__ int key(int v) const { return owner(v) * per + local(v); }
+  __device__ __forceinline__ int total() const { return start[(int64_t)per << g]; }
 };
 
+template <int KIND>
 __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   ::tp::pdl_enter();
   extern __shared__ int32_t sort_sm[];
-  __shared__ int32_t sh[SORT_WARPS], hits[SORT_WARPS][64];
+  __shared__ int32_t sh[SORT_WARPS];
   const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
   int32_t* count = sort_sm;                                  // [warps][W]
-  uint32_t* words = (uint32_t*)(sort_sm + SORT_WARPS * W);   // hits of 32 positions each
+  uint16_t* hits = (uint16_t*)(sort_sm + SORT_WARPS * W);    // [warps][1024]
+  uint32_t* words = (uint32_t*)(hits + SORT_WARPS * 1024);   // hits of 32 positions each
   const int64_t nwords = (e.n + 31) >> 5;
   const bool kept = nwords <= SORT_WORDS;
   const int64_t per = (nwords + SORT_WARPS - 1) / SORT_WARPS;  // words of one warp: neighbours, so that order is kept
@@ -156,23 +169,29 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   __syncthreads();
   auto token = [&](int64_t word) {
     const int64_t p = word * 32 + lane;
-    return word < w1 && p < e.n ? token_id(e.ids, e.kind, p) : -1;
+    return word < w1 && p < e.n ? token_id(e.ids, KIND, p) : -1;
   };
   int less = 0;
   for (int64_t i = w0; i < w1; i += SORT_U) {
     int v[SORT_U];
+    uint32_t mine = 0u;
+    if (i + SORT_U <= w1 && (i + SORT_U) * 32 <= e.n) {
+      const int32_t* at = static_cast<const int32_t*>(e.ids) + i * 32 + lane;  // either storage is 4 bytes
 #pragma unroll
-    for (int q = 0; q < SORT_U; ++q) v[q] = token(i + q);
+      for (int q = 0; q < SORT_U; ++q) v[q] = token_id(at + 32 * q, KIND, 0);
+    } else {
+#pragma unroll
+      for (int q = 0; q < SORT_U; ++q) v[q] = token(i + q);
+    }
 #pragma unroll
     for (int q = 0; q < SORT_U; ++q) {
-      const bool ok = e.valid(v[q]);
-      const int local = (int)e.ctas.div(ok ? (uint32_t)v[q] : 0u), owner = v[q] - local * (int)e.ctas.d;
-      less += ok && owner < me;
-      const bool hit = ok && owner == me;
-      if (hit) atomicAdd(&count[w * W + local], 1);
+      const bool ok = e.valid(v[q]), hit = ok && e.owner(v[q]) == me;
+      less += ok && e.owner(v[q]) < me;
       const uint32_t b = __ballot_sync(0xffffffffu, hit);
-      if (kept && lane == 0 && i + q < w1) words[i + q] = b;
+      if (hit) atomicAdd(&count[w * W + e.local(v[q])], 1);
+      mine = lane == q ? b : mine;
     }
+    if (kept && lane < SORT_U && i + lane < w1) words[i + lane] = mine;
   }
   for (int o = 16; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
   if (lane == 0) sh[w] = less;
@@ -208,184 +227,243 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
     if (me == (int)gridDim.x - 1 && t == W - 1) e.start[(int64_t)gridDim.x * W] = first + c;
   }
   __syncthreads();
-  // Positions of hits, in order, 32 at a time: a lane each.
-  int32_t* buf = hits[w];
-  int have = 0;
-  auto place = [&](int k) {  // the first k of buf
-    __syncwarp();
-    const uint32_t some = k == 32 ? 0xffffffffu : (1u << k) - 1;
-    if (lane < k) {
-      const int p = buf[lane], v = token_id(e.ids, e.kind, p), local = (int)e.ctas.div((uint32_t)v);
-      const uint32_t peers = __match_any_sync(some, local);
-      const int rank = __popc(peers & ((1u << lane) - 1)), at = count[w * W + local];
-      __syncwarp(some);
-      if (rank == 0) count[w * W + local] = at + __popc(peers);
-      e.pos[at + rank] = p;
-      e.tok[at + rank] = v;
-    }
-    __syncwarp();
-  };
-  auto take = [&](int64_t word, uint32_t b) {
-    if (b >> lane & 1) buf[have + __popc(b & ((1u << lane) - 1))] = (int32_t)(word * 32 + lane);
-    have += __popc(b);
-    if (have >= 32) {
-      place(32);
-      const int32_t rest = buf[32 + lane];
-      __syncwarp();
-      buf[lane] = rest;
-      have -= 32;
-      __syncwarp();
-    }
-  };
-  if (kept) {
-    for (int64_t i = w0; i < w1; i += 32) {
-      const uint32_t mine = i + lane < w1 ? words[i + lane] : 0u;
-      for (uint32_t some = __ballot_sync(0xffffffffu, mine != 0u); some; some &= some - 1) {
-        const int j = __ffs(some) - 1;
-        take(i + j, __shfl_sync(0xffffffffu, mine, j));
+  // 32 words at a time: a lane lists its word's hits, in order, as offsets from the
+  // first word's position; then the hits are placed 32 at a time, a lane each, the
+  // tokens of the next 32 under way.
+  uint16_t* list = hits + 1024 * w;
+  for (int64_t i = w0; i < w1; i += 32) {
+    uint32_t mine = 0u;
+    if (kept) {
+      if (i + lane < w1) mine = words[i + lane];
+    } else {
+      for (int j = 0; j < 32; ++j) {
+        const int v = token(i + j);
+        const uint32_t b = __ballot_sync(0xffffffffu, e.valid(v) && e.owner(v) == me);
+        if (lane == j) mine = b;
       }
     }
-  } else {
-    for (int64_t i = w0; i < w1; ++i) {
-      const int v = token(i);
-      const bool ok = e.valid(v);
-      take(i, __ballot_sync(0xffffffffu, ok && (int)e.ctas.mod(ok ? (uint32_t)v : 0u) == me));
+    int at = __popc(mine);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += u;
+    }
+    const int have = __shfl_sync(0xffffffffu, at, 31);
+    at -= __popc(mine);
+    for (; mine; mine &= mine - 1) list[at++] = (uint16_t)(32 * lane + __ffs(mine) - 1);
+    __syncwarp();
+    const int64_t first = i * 32;
+    auto fetch = [&](int h) { return h < have ? token_id(e.ids, KIND, first + list[h]) : 0; };
+    int v = fetch(lane);
+    for (int h = 0; h < have; h += 32) {
+      const int next = fetch(h + 32 + lane), k = have - h < 32 ? have - h : 32;
+      if (lane < k) {
+        const uint32_t some = k == 32 ? 0xffffffffu : (1u << k) - 1;
+        int32_t* c = &count[w * W + e.local(v)];
+        const uint32_t peers = __match_any_sync(some, v);
+        const int rank = __popc(peers & ((1u << lane) - 1)), to = *c;
+        __syncwarp(some);
+        if (rank == 0) *c = to + __popc(peers);
+        e.pos[to + rank] = (int32_t)(first + list[h + lane]);
+        e.tok[to + rank] = v;
+      }
+      __syncwarp();
+      v = next;
     }
   }
-  if (have) place(have);
 }
 
-// Tiles of SUM_T sorted positions are summed each by itself, so a frequent
-// token takes no longer than many rare ones.  A run (the positions of one token)
-// of at most SUM_RUN goes whole to the tile it starts in.  A longer one is cut
-// at the tiles' borders: what came in from the tile before is the tile's
-// partial 0, the start of what goes on its partial 1 (what does both, partial 0).
-constexpr int SUM_T = 64, SUM_RUN = 128;
-constexpr int SUM_ZERO = 4;  // rows without a token that a thread clears
+// Tiles of T sorted positions are summed each by itself, so a frequent token
+// takes no longer than many rare ones.  A run (the positions of one token) of at
+// most 2 T goes whole to the tile it starts in.  A longer one is cut at the
+// tiles' borders: what came in from the tile before is the tile's partial 0, the
+// start of what goes on its partial 1 (what does both, partial 0).  T is 64, or
+// 16 where 64 would leave SMs without a tile.
+struct EmbedSum {
+  const float* dout;
+  int64_t ldo, cols;
+  int chunks, T;
+  int64_t tiles, tile_ctas;
+  float scale;
+  float* dtable;
+  int64_t ld;
+  float* partial;  // [2 tiles][ldp]
+  int64_t ldp;
+  int2* cut;       // [tiles]: the cut run that starts in a tile: its token (-1: none) and its last tile
+};
 
-template <int VEC, bool ACC>
-__global__ void __launch_bounds__(EMB_NT) k_embed_sum(const EmbedSort e, const float* __restrict__ dout, int64_t ldo,
-                                                      int64_t cols, int chunks, int64_t tiles, int64_t tile_ctas,
-                                                      float scale, float* __restrict__ dtable, int64_t ld,
-                                                      float* __restrict__ partial, int64_t ldp,
-                                                      int2* __restrict__ cut) {
-  ::tp::pdl_enter();
-  const int64_t group = blockIdx.x / chunks;
-  const int64_t c = (int64_t)(blockIdx.x - group * chunks) * blockDim.x + threadIdx.x;
-  if (c >= cols) return;
-  if (group >= tile_ctas) {  // rows whose token is absent
-    const int64_t v0 = ((group - tile_ctas) * blockDim.y + threadIdx.y) * SUM_ZERO;
-#pragma unroll
-    for (int r = 0; r < SUM_ZERO; ++r) {
-      const int64_t v = v0 + r;
-      if (v >= e.V) return;
+constexpr int SUM_U = 8;     // rows in flight per thread (two 16-byte vectors of positions)
+constexpr int SUM_ZERO = 4;  // rows looked at by a warp (or thread) that clears those of absent tokens
+
+template <int VEC>
+__device__ __forceinline__ void embed_zero(const EmbedSort& e, const EmbedSum& a, int64_t group) {
+  if (blockDim.x < 32) {  // narrow rows: a thread per column
+    const int64_t v0 = (group * blockDim.y + threadIdx.y) * SUM_ZERO;
+    if (threadIdx.x >= a.cols) return;
+    for (int64_t v = v0; v < v0 + SUM_ZERO && v < e.V; ++v) {
       const int k = e.key((int)v);
-      if (e.start[k] == e.start[k + 1]) Col<VEC>::zero().store(dtable + v * ld, c);
+      if (e.start[k] == e.start[k + 1]) Col<VEC>::zero().store(a.dtable + v * a.ld, threadIdx.x);
     }
     return;
   }
-  const int64_t tile = group * blockDim.y + threadIdx.y;
-  const int m = e.total();
-  int2 starts = make_int2(-1, 0);  // the cut run that starts here: its token, its last tile
-  if (tile * SUM_T >= m) {
-    if (c == 0 && tile < tiles) cut[tile] = starts;
+  // a warp per row, in 16-byte stores between its ends
+  const int t = threadIdx.y * blockDim.x + threadIdx.x, lane = t & 31;
+  const int64_t v0 = (group * (EMB_NT / 32) + (t >> 5)) * SUM_ZERO, D = a.cols * VEC;
+  bool gone = false;
+  if (lane < SUM_ZERO && v0 + lane < e.V) {
+    const int k = e.key((int)(v0 + lane));
+    gone = e.start[k] == e.start[k + 1];
+  }
+  for (uint32_t some = __ballot_sync(0xffffffffu, gone); some; some &= some - 1) {
+    float* row = a.dtable + (v0 + __ffs(some) - 1) * a.ld;
+    int64_t head = (4 - (((uintptr_t)row >> 2) & 3)) & 3;
+    if (head > D) head = D;
+    const int64_t body = (D - head) >> 2;
+    if (lane < head) row[lane] = 0.0f;
+    float4* mid = reinterpret_cast<float4*>(row + head);
+#pragma unroll 4
+    for (int64_t q = lane; q < body; q += 32) mid[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (lane < D - head - 4 * body) row[head + 4 * body + lane] = 0.0f;
+  }
+}
+
+// (4 CTAs to an SM with the old values in flight: 136 registers would leave 3, and
+// 65536 x 1024 then takes 116 us instead of 104; 8 would spill, 181 us.)
+template <int VEC, bool ACC>
+__global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(const EmbedSort e, const EmbedSum a) {
+  ::tp::pdl_enter();
+  if (blockIdx.x >= a.tile_ctas * a.chunks) {
+    embed_zero<VEC>(e, a, blockIdx.x - a.tile_ctas * a.chunks);
     return;
   }
-  const int s0 = (int)(tile * SUM_T);
-  int s1 = m - s0 < SUM_T ? m : s0 + SUM_T, from = s0;
-  int cur = e.tok[s0];
+  const int64_t group = blockIdx.x / a.chunks;
+  const int64_t c = (int64_t)(blockIdx.x - group * a.chunks) * blockDim.x + threadIdx.x;
+  const int64_t tile = group * blockDim.y + threadIdx.y;
+  if (c >= a.cols || tile >= a.tiles) return;
+  const int T = a.T, m = e.total();
+  int2 starts = make_int2(-1, 0);
+  if (tile * T >= m) {
+    if (c == 0) a.cut[tile] = starts;
+    return;
+  }
+  const int s0 = (int)(tile * T);
+  int s1 = m - s0 < T ? m : s0 + T, from = s0;
+  const int first = e.tok[s0], before = s0 > 0 ? e.tok[s0 - 1] : -1;
+  const int final = e.tok[s1 - 1], after = s1 < m ? e.tok[s1] : -1;
   bool came_in = false, goes_on = false;
-  if (s0 > 0 && e.tok[s0 - 1] == cur) {
-    const int k = e.key(cur), end = e.start[k + 1];
-    if (end - e.start[k] > SUM_RUN) came_in = true;
+  if (before == first) {
+    const int k = e.key(first), end = e.start[k + 1];
+    if (end - e.start[k] > 2 * T) came_in = true;
     else from = end;
   }
-  if (s1 < m) {
-    const int v = e.tok[s1 - 1];
-    if (e.tok[s1] == v) {
-      const int k = e.key(v), end = e.start[k + 1];
-      if (end - e.start[k] > SUM_RUN) {
-        goes_on = true;
-        if (e.start[k] >= s0) starts = make_int2(v, (end - 1) / SUM_T);
-      } else if (e.start[k] >= s0) {
-        s1 = end;
-      }
+  if (after == final) {
+    const int k = e.key(final), start = e.start[k], end = e.start[k + 1];
+    if (end - start > 2 * T) {
+      goes_on = true;
+      if (start >= s0) starts = make_int2(final, (end - 1) / T);
+    } else if (start >= s0) {
+      s1 = end;
     }
   }
-  if (c == 0) cut[tile] = starts;
+  if (c == 0) a.cut[tile] = starts;
   if (from >= s1) return;  // all of it belongs to a run of the tile before
-  cur = e.tok[from];
-  float* part = partial + 2 * tile * ldp;
+  int cur = e.tok[from];
+  float* part = a.partial + 2 * tile * a.ldp;
   Col<VEC> acc = Col<VEC>::zero();
-  auto flush = [&]() {
+  auto flush = [&](const Col<VEC>& old) {
     if (came_in) {
       acc.store(part, c);
     } else {
-      float* row = dtable + (int64_t)cur * ld;
-      Col<VEC> r = acc.times(scale);
-      if (ACC) r.add(Col<VEC>::load(row, c));
-      r.store(row, c);
+      Col<VEC> r = acc.times(a.scale);
+      if (ACC) r.add(old);
+      r.store(a.dtable + (int64_t)cur * a.ld, c);
     }
   };
-  for (int s = from; s < s1; s += 8) {
-    int tok[8];
-    Col<VEC> x[8];
+  // eight positions at a time, on eight-position boundaries (one past the last is
+  // still inside the workspace); lo, hi: which of them are the tile's
+  auto batch = [&](int s, int lo, int hi) {
+    const int4 t0 = *reinterpret_cast<const int4*>(e.tok + s), t1 = *reinterpret_cast<const int4*>(e.tok + s + 4);
+    const int4 p0 = *reinterpret_cast<const int4*>(e.pos + s), p1 = *reinterpret_cast<const int4*>(e.pos + s + 4);
+    const int tok[SUM_U] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
+    const int pos[SUM_U] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+    Col<VEC> x[SUM_U], old[ACC ? SUM_U : 1];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (s + k < s1) {
-        tok[k] = e.tok[s + k];
-        x[k] = Col<VEC>::load(dout + (int64_t)e.pos[s + k] * ldo, c);
-      }
+    for (int k = 0; k < SUM_U; ++k)
+      if (k >= lo && k < hi) x[k] = Col<VEC>::load(a.dout + (int64_t)pos[k] * a.ldo, c);
+    if (ACC)  // the rows that runs ending in this batch are added to (each is this thread's alone)
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (s + k < s1) {
+      for (int k = 0; k < SUM_U; ++k)
+        if (k >= lo && k < hi) {
+          const int prev = k > lo ? tok[k > 0 ? k - 1 : 0] : cur;
+          if (tok[k] != prev) old[k] = Col<VEC>::load(a.dtable + (int64_t)prev * a.ld, c);
+        }
+#pragma unroll
+    for (int k = 0; k < SUM_U; ++k)
+      if (k >= lo && k < hi) {
         if (tok[k] != cur) {
-          flush();
+          flush(old[ACC ? k : 0]);
           cur = tok[k];
           came_in = false;
           acc = Col<VEC>::zero();
         }
         acc.add(x[k]);
       }
+  };
+  int s = from & ~(SUM_U - 1);
+  if (s < from) {
+    batch(s, from - s, s1 - s < SUM_U ? s1 - s : SUM_U);
+    s += SUM_U;
   }
-  if (!came_in && goes_on) acc.store(part + ldp, c);
-  else flush();
+  for (; s + SUM_U <= s1; s += SUM_U) batch(s, 0, SUM_U);
+  if (s < s1) batch(s, 0, s1 - s);
+  if (!came_in && goes_on) {
+    acc.store(part + a.ldp, c);
+  } else {
+    Col<VEC> old;
+    if (ACC && !came_in) old = Col<VEC>::load(a.dtable + (int64_t)cur * a.ld, c);
+    flush(old);
+  }
 }
 
 // The runs that were cut: the tile one starts in adds up its partial 1 and the
 // partials 0 of the tiles after it, in f64: eight threads take every eighth,
-// and their sums are added in order.  A CTA looks through 32 tiles for such starts.
-constexpr int JOIN_COLS = 32, JOIN_ROWS = 8;
+// and their sums are added in order.  A CTA looks through 8 tiles for such starts.
+constexpr int JOIN_TILES = 8, JOIN_ROWS = 8;
 
 template <bool ACC>
-__global__ void __launch_bounds__(JOIN_COLS* JOIN_ROWS) k_embed_join(const int2* __restrict__ cut,
-                                                                     int64_t tiles, int64_t D, int chunks,
-                                                                     float scale, float* __restrict__ dtable,
-                                                                     int64_t ld, const float* __restrict__ partial,
-                                                                     int64_t ldp) {
+__global__ void __launch_bounds__(32 * JOIN_ROWS) k_embed_join(const EmbedSum a, int64_t D, int chunks) {
   ::tp::pdl_enter();
-  __shared__ double sh[JOIN_ROWS][JOIN_COLS];
+  __shared__ double sh[JOIN_ROWS][4][32];
+  const int lane = threadIdx.x, r = threadIdx.y;
   const int64_t group = blockIdx.x / chunks;
-  const int64_t c = (int64_t)(blockIdx.x - group * chunks) * JOIN_COLS + threadIdx.x;
-  const int64_t mine = group * 32 + threadIdx.x;  // every warp looks at the same 32 tiles
-  const int2 run = mine < tiles ? cut[mine] : make_int2(-1, 0);
+  const int64_t c4 = (int64_t)(blockIdx.x - group * chunks) * 32 + lane;  // a 4-value column of the partials
+  const int64_t mine = group * JOIN_TILES + lane;                         // every warp looks at the same tiles
+  const int2 run = lane < JOIN_TILES && mine < a.tiles ? a.cut[mine] : make_int2(-1, 0);
   for (uint32_t some = __ballot_sync(0xffffffffu, run.x >= 0); some; some &= some - 1) {
     const int which = __ffs(some) - 1;
-    const int64_t tile = group * 32 + which;
+    const int64_t tile = group * JOIN_TILES + which;
     const int v = __shfl_sync(0xffffffffu, run.x, which), last = __shfl_sync(0xffffffffu, run.y, which);
-    double acc = 0.0;
-    if (c < D) {
-      if (threadIdx.y == 0) acc = partial[(2 * tile + 1) * ldp + c];
-#pragma unroll 8
-      for (int64_t k = tile + 1 + threadIdx.y; k <= last; k += JOIN_ROWS) acc += partial[2 * k * ldp + c];
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    auto add = [&](int64_t row) {
+      const float4 x = *(reinterpret_cast<const float4*>(a.partial + row * a.ldp) + c4);
+      acc[0] += x.x;
+      acc[1] += x.y;
+      acc[2] += x.z;
+      acc[3] += x.w;
+    };
+    if (4 * c4 < D) {
+      if (r == 0) add(2 * tile + 1);
+#pragma unroll 4
+      for (int64_t k = tile + 1 + r; k <= last; k += JOIN_ROWS) add(2 * k);
     }
-    sh[threadIdx.y][threadIdx.x] = acc;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sh[r][q][lane] = acc[q];
     __syncthreads();
-    if (threadIdx.y == 0 && c < D) {
-      for (int r = 1; r < JOIN_ROWS; ++r) acc += sh[r][threadIdx.x];
-      float* row = dtable + (int64_t)v * ld;
-      const float g = (float)(acc * scale);
-      row[c] = ACC ? row[c] + g : g;
+    if (r < 4) {  // warp r: value r of each column
+      double sum = 0.0;
+      for (int i = 0; i < JOIN_ROWS; ++i) sum += sh[i][r][lane];
+      const float g = (float)(sum * a.scale);
+      float* row = a.dtable + (int64_t)v * a.ld + 4 * c4 + r;
+      if (4 * c4 + r < D) *row = ACC ? *row + g : g;
     }
     __syncthreads();
   }
@@ -411,22 +489,21 @@ void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int
   else TP_LAUNCH(k_embed<1>, grid, dim3(tx, ty), 0, table, ld, ids, kind, n, V, cols, chunks, scale, out, ldo);
 }
 
-// Up to this many tokens are added to an existing gradient without sorting.
-constexpr int64_t EMB_FEW = 2048;
-
 struct EmbedPlan {
-  int64_t ctas, per, start, pos, tok, cut, partial, ldp, bytes, tiles;
+  int64_t per, start, pos, tok, cut, partial, ldp, bytes, tiles;
+  int g, T;
   EmbedPlan(int64_t n, int64_t V, int64_t D) {
-    const int64_t sms = 148, waves = (V + sms * SORT_TOKENS - 1) / (sms * SORT_TOKENS);
-    ctas = V < sms * waves ? V : sms * waves;
-    per = (V + ctas - 1) / ctas;
-    tiles = (n + SUM_T - 1) / SUM_T;
+    g = 7;  // 128 CTAs for 148 SMs
+    while (((int64_t)SORT_TOKENS << g) < V) ++g;
+    per = (V + (1 << g) - 1) >> g;
+    T = n / 64 * D >= 148 * 8 * 512 ? 64 : 16;  // 512 values of a row to a CTA, 8 CTAs to an SM
+    tiles = (n + T - 1) / T;
     ldp = (D + 3) / 4 * 4;
     auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
     start = 0;
-    pos = start + up((ctas * per + 1) * 4);
-    tok = pos + up(n * 4);
-    cut = tok + up(n * 4);
+    pos = start + up(((per << g) + 1) * 4);
+    tok = pos + up(n * 4 + 32);
+    cut = tok + up(n * 4 + 32);
     partial = cut + up(tiles * 8);
     bytes = partial + 2 * tiles * ldp * 4;
   }
@@ -435,62 +512,72 @@ struct EmbedPlan {
 int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return EmbedPlan(n, V, D).bytes; }
 
 template <int VEC, bool ACC>
-static void launch_sum(const EmbedPlan& p, const EmbedSort& e, const float* dout, int64_t ldo, int64_t D, float scale,
-                       float* dtable, int64_t ld, float* partial, int2* cut) {
+static void launch_sum(const EmbedSort& e, EmbedSum a, int64_t D) {
   const char* what = "token_embedding_backward";
-  const int64_t cols = VEC == 4 ? D / 4 : D;
-  const int tx = block_cols(cols), ty = EMB_NT / tx;
-  const int chunks = (int)((cols + tx - 1) / tx);
-  const int64_t tile_ctas = (p.tiles + ty - 1) / ty;
-  const int64_t zero_ctas = ACC ? 0 : ((int64_t)e.V + ty * SUM_ZERO - 1) / (ty * SUM_ZERO);
-  const unsigned grid = grid_of(tile_ctas + zero_ctas, chunks, what);
-  if (grid == 0) return;
-  TP_LAUNCH((k_embed_sum<VEC, ACC>), grid, dim3(tx, ty), 0, e, dout, ldo, cols, chunks, p.tiles, tile_ctas, scale,
-            dtable, ld, partial, p.ldp, cut);
-  if (p.tiles < 2) return;  // nothing crosses
-  const int jchunks = (int)((D + JOIN_COLS - 1) / JOIN_COLS);
-  TP_LAUNCH(k_embed_join<ACC>, grid_of((p.tiles + 31) / 32, jchunks, what), dim3(JOIN_COLS, JOIN_ROWS), 0,
-            cut, p.tiles, D, jchunks, scale, dtable, ld, partial, p.ldp);
+  a.cols = VEC == 4 ? D / 4 : D;
+  const int tx = block_cols(a.cols), ty = EMB_NT / tx;
+  a.chunks = (int)((a.cols + tx - 1) / tx);
+  a.tile_ctas = (a.tiles + ty - 1) / ty;
+  const int64_t rows = (tx < 32 ? ty : EMB_NT / 32) * SUM_ZERO;  // of one clearing CTA
+  const int64_t zero_ctas = ACC ? 0 : (e.V + rows - 1) / rows;
+  const int64_t grid = (int64_t)grid_of(a.tile_ctas, a.chunks, what) + zero_ctas;
+  TP_REQUIRE(grid <= INT_MAX, "%s: too many tokens, rows or columns for one launch", what);
+  TP_LAUNCH((k_embed_sum<VEC, ACC>), (unsigned)grid, dim3(tx, ty), 0, e, a);
+  if (a.tiles < 2) return;  // nothing is cut
+  const int jchunks = (int)((D + 127) / 128);
+  TP_LAUNCH(k_embed_join<ACC>, grid_of((a.tiles + JOIN_TILES - 1) / JOIN_TILES, jchunks, what), dim3(32, JOIN_ROWS), 0,
+            a, D, jchunks);
 }
 
 void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
                       float scale, int64_t pad, bool accumulate, float* dtable, int64_t ld, void* ws) {
   if (D == 0 || (n == 0 && accumulate)) return;
+  const bool vec = D % 4 == 0 && aligned_rows(dout, ldo) && aligned_rows(dtable, ld);
   if (accumulate && n <= EMB_FEW) {
-    const int chunks = (int)((D + 255) / 256);
-    TP_LAUNCH(k_embed_bwd_few, grid_of(n, chunks, "token_embedding_backward"), 256, 0, dout, ldo, ids, kind, (int)n, V,
-              D, chunks, scale, pad, dtable, ld);
+    const int64_t cols = vec ? D / 4 : D;
+    const int chunks = (int)((cols + 255) / 256);
+    const unsigned grid = grid_of(n, chunks, "token_embedding_backward");
+    if (vec) TP_LAUNCH(k_embed_few<4>, grid, 256, 0, dout, ldo, ids, kind, (int)n, V, cols, chunks, scale, pad, dtable, ld);
+    else TP_LAUNCH(k_embed_few<1>, grid, 256, 0, dout, ldo, ids, kind, (int)n, V, cols, chunks, scale, pad, dtable, ld);
     return;
   }
   const EmbedPlan p(n, V, D);
   char* base = (char*)ws;
   EmbedSort e;
-  e.ctas = fast_div((uint32_t)p.ctas);
+  e.g = p.g;
   e.per = (int)p.per;
   e.n = n;
   e.V = (int)V;
   e.pad = (int)pad;
-  e.kind = kind;
   e.ids = ids;
   e.start = (int32_t*)(base + p.start);
   e.pos = (int32_t*)(base + p.pos);
   e.tok = (int32_t*)(base + p.tok);
-  float* partial = (float*)(base + p.partial);
-  int2* cut = (int2*)(base + p.cut);
   const int64_t words = (n + 31) / 32;
-  const size_t smem = (size_t)(SORT_WARPS * p.per + (words <= SORT_WORDS ? words : 0)) * 4;
-  static bool raised = false;
-  if (!raised) {  // 64 KB of counts and 128 KB of hits at most
-    TP_CUDA(cudaFuncSetAttribute(k_embed_sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (SORT_WARPS * SORT_TOKENS + SORT_WORDS) * 4));
-    raised = true;
+  const size_t smem = (size_t)(SORT_WARPS * p.per + SORT_WARPS * 512 + (words <= SORT_WORDS ? words : 0)) * 4;
+  auto sort = kind == IDS_I32 ? k_embed_sort<IDS_I32> : k_embed_sort<IDS_F32>;
+  static bool raised[2] = {false, false};
+  if (!raised[kind]) {  // 64 KB each of counts, listed hits and hits at most
+    TP_CUDA(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (SORT_WARPS * (SORT_TOKENS + 512) + SORT_WORDS) * 4));
+    raised[kind] = true;
   }
-  TP_LAUNCH(k_embed_sort, (unsigned)p.ctas, SORT_NT, smem, e);
-  const bool vec = D % 4 == 0 && aligned_rows(dout, ldo) && aligned_rows(dtable, ld);
-  if (vec && accumulate) launch_sum<4, true>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
-  else if (vec) launch_sum<4, false>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
-  else if (accumulate) launch_sum<1, true>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
-  else launch_sum<1, false>(p, e, dout, ldo, D, scale, dtable, ld, partial, cut);
+  TP_LAUNCH(sort, 1u << p.g, SORT_NT, smem, e);
+  EmbedSum a;
+  a.dout = dout;
+  a.ldo = ldo;
+  a.T = p.T;
+  a.tiles = p.tiles;
+  a.scale = scale;
+  a.dtable = dtable;
+  a.ld = ld;
+  a.partial = (float*)(base + p.partial);
+  a.ldp = p.ldp;
+  a.cut = (int2*)(base + p.cut);
+  if (vec && accumulate) launch_sum<4, true>(e, a, D);
+  else if (vec) launch_sum<4, false>(e, a, D);
+  else if (accumulate) launch_sum<1, true>(e, a, D);
+  else launch_sum<1, false>(e, a, D);
 }
 
 static void check_embed(int64_t n, int64_t V, int64_t D, int64_t ld, int64_t ldo, const char* what) {
