@@ -128,6 +128,15 @@ def test_gradient_of_long_sums(cuda_rt):
     check_grad(cuda_rt, rng.standard_normal((n, 3)), ids, 500, 0.5, old=rng.standard_normal((500, 3)).astype(np.float32))
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_of_many_tokens(cuda_rt, accumulate):
+    """More positions than the sort keeps hits of in shared memory."""
+    rng = np.random.default_rng(17)
+    n, V = 600001, 3000
+    old = rng.standard_normal((V, 2)).astype(np.float32) if accumulate else None
+    check_grad(cuda_rt, rng.standard_normal((n, 2)), zipf(rng, n, V), V, 1.0, pad=7, old=old)
+
+
 @pytest.mark.parametrize("V", [1, 149, 100000, 2 ** 20])
 def test_gradient_vocabularies(cuda_rt, V):
     rng = np.random.default_rng(V)

@@ -147,13 +147,12 @@ def embed_grad(dout, ids, V, scale, pad, old=None):
     results added with at most as many roundings again, one product by the
     scale and one addition to the old value."""
     D = dout.shape[1]
+    ids = np.asarray(ids)
     g, a, cnt = np.zeros((V, D)), np.zeros((V, D)), np.zeros(V)
-    for i, v in enumerate(ids):
-        v = int(v)
-        if 0 <= v < V and v != pad:
-            g[v] += dout[i].astype(np.float64)
-            a[v] += np.abs(dout[i])
-            cnt[v] += 1
+    keep = (ids >= 0) & (ids < V) & (ids != pad)
+    np.add.at(g, ids[keep].astype(np.int64), dout[keep].astype(np.float64))
+    np.add.at(a, ids[keep].astype(np.int64), np.abs(dout[keep]).astype(np.float64))
+    np.add.at(cnt, ids[keep].astype(np.int64), 1.0)
     s = float(np.float32(scale))
     g, a = g * s, a * abs(s)
     tol = U * (np.minimum(cnt, 256)[:, None] + 3) * a
