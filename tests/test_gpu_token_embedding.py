@@ -2,6 +2,9 @@
 forward is one product, rounded once; the gradient's bound counts the roundings
 of its sums (token_oracle.embed_grad)."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -174,6 +177,74 @@ def test_gradient_equal_inputs_equal_bits(cuda_rt):
         a = grad(cuda_rt, dout, ids, V, 1.0)
         for _ in range(3):
             assert np.array_equal(a, grad(cuda_rt, dout, ids, V, 1.0))
+
+
+def test_offsets_beyond_32_bits(cuda_rt):
+    """Rows of table, output and gradient 1.1 * 10^9 values apart."""
+    rt = cuda_rt
+    ld, D, V = 1100000000, 8, 3
+    p = ctypes.c_void_p()
+    assert rt.lib.tp_alloc((2 * ld + D) * 4, ctypes.byref(p)) == 0
+    table = np.random.default_rng(3).standard_normal((V, D)).astype(np.float32)
+
+    def rows(put=None):
+        out = np.zeros((V, D), np.float32)
+        for r in range(V):
+            if put is not None:
+                assert rt.lib.tp_memcpy_h2d(p.value + 4 * ld * r, put[r].ctypes.data_as(ctypes.c_void_p), 4 * D) == 0
+            else:
+                assert rt.lib.tp_memcpy_d2h(out[r].ctypes.data_as(ctypes.c_void_p), p.value + 4 * ld * r, 4 * D) == 0
+        return out
+
+    rows(table)
+    ids = np.array([2, 0, 2, 1], np.int32)
+    I, O = Buf(rt, ids), Buf(rt, np.zeros((4, D), np.float32))
+    assert rt.lib.tpk_token_embedding(p.value, ld, I.ptr, 1, 4, V, D, 1.0, O.ptr, D) == 0
+    assert np.array_equal(O.read(), table[ids])
+    W = Buf(rt, np.zeros(1 << 16, np.uint8))
+    for acc, want in ((1, 2 * table), (0, table)):  # a table's rows come back as their gradient
+        want = want.copy()
+        want[2] += table[2]
+        assert rt.lib.tpk_token_embedding_backward(O.ptr, D, I.ptr, 1, 4, V, D, 1.0, -1, acc, p.value, ld, W.ptr,
+                                                   1 << 16) == 0
+        assert np.allclose(rows(), want, rtol=4 * U)
+    J = Buf(rt, np.array([0, 1, 1], np.int32))
+    R = Buf(rt, np.zeros((V, D), np.float32))
+    rows(table)
+    assert rt.lib.tpk_token_embedding_backward(p.value, ld, J.ptr, 1, 3, V, D, 1.0, -1, 0, R.ptr, D, W.ptr, 1 << 16) == 0
+    assert np.allclose(R.read(), [table[0], table[1] + table[2], 0 * table[0]], rtol=4 * U)
+    assert rt.lib.tp_free(p.value) == 0
+
+
+def test_first_call_inside_a_capture():
+    """In a fresh process the first gradient is captured, not run."""
+    code = """
+import ctypes, sys
+import numpy as np
+sys.path[:0] = [%r, %r]
+from tpcuda import CudaRuntime
+from token_oracle import Buf, embed_grad
+rt = CudaRuntime()
+rng = np.random.default_rng(0)
+n, V, D = 3000, 500, 20
+dout, ids = rng.standard_normal((n, D)).astype(np.float32), rng.integers(0, V, n).astype(np.int32)
+need = ctypes.c_int64()
+assert rt.lib.tpk_token_embedding_backward_ws(n, V, D, ctypes.byref(need)) == 0
+G, I, T, W = (Buf(rt, a) for a in (dout, ids, np.zeros((V, D), np.float32), np.zeros(need.value, np.uint8)))
+assert rt.lib.tp_graph_begin() == 0
+assert rt.lib.tpk_token_embedding_backward(G.ptr, D, I.ptr, 1, n, V, D, 1.0, -1, 0, T.ptr, D, W.ptr, need.value) == 0
+g = ctypes.c_int64()
+assert rt.lib.tp_graph_end(ctypes.byref(g)) == 0, rt.lib.tp_last_error()
+for _ in range(2):
+    assert rt.lib.tp_graph_launch(g.value) == 0
+want, tol = embed_grad(dout, ids, V, 1.0, -1)
+assert np.all(np.abs(T.read() - want) <= tol)
+print("captured")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = code % (os.path.join(os.path.dirname(here), "torch-pyodide_b200"), here)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_gradient_empty_batch(cuda_rt):

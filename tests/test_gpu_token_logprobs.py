@@ -3,6 +3,8 @@
 Tolerances: token_oracle.logprobs_tolerance and logprobs_grad give, per value,
 the sum of the roundings that any one-pass f32 evaluation of the formulas
 makes; ids are compared exactly (equal logits: the lower id first)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -160,24 +162,85 @@ def test_float_ids_are_truncated(cuda_rt):
     assert L.read()[3] == 0.0
 
 
+def pattern(shape, V, K, rng):
+    i, small = np.arange(V), rng.standard_normal(V)
+    if shape == "threads over":  # all but one of K threads' columns hold larger values than its best
+        row = np.where((i // 4) % 256 < K, 20 + small, np.minimum(small, 3))
+        return np.where((i // 4) % 256 == K - 1, 5.0 + 0.01 * small, row)
+    if shape == "lanes over":
+        row = np.where((i // 4) % 32 < K, 20 + small, np.minimum(small, 3))
+        return np.where((i // 4) % 32 == K - 1, 5.0 + 0.01 * small, row)
+    return {"equal": np.zeros(V), "rising": i * 1e-3, "falling": -i * 1e-3, "two values": (i % 7 == 3) * 1.0,
+            "few values": np.floor(small * 2), "columns": np.where((i // 4) % 256 == 17, 10 + rng.random(V), small),
+            "blocks": np.where(i // 1024 == (V // 1024) // 2, 10 + small, small),
+            "tail": np.where(i >= V - K, 9.0 + i * 1e-5, small), "head": np.where(i < 3, 9.0, small),
+            "normal": small}[shape]
+
+
+SHAPES = ["equal", "rising", "falling", "two values", "few values", "columns", "blocks", "threads over", "lanes over",
+          "tail", "head"]
+
+
 @pytest.mark.parametrize("V", [600, 4096, 40000, 140001])
 @pytest.mark.parametrize("K", [1, 20, 32])
-@pytest.mark.parametrize("shape", ["equal", "rising", "falling", "two values", "few values", "columns", "blocks",
-                                   "threads over", "tail", "head"])
+@pytest.mark.parametrize("shape", SHAPES)
 def test_alternatives_wherever_they_stand(cuda_rt, V, K, shape):
     """Rows whose largest logits sit where a split of the row over threads and
     CTAs could lose them: ties, runs, one thread's columns, one block."""
     rng = np.random.default_rng(V + K)
-    i = np.arange(V)
-    small = rng.standard_normal(V)
-    row = {"equal": np.zeros(V), "rising": i * 1e-3, "falling": -i * 1e-3, "two values": (i % 7 == 3) * 1.0,
-           "few values": np.floor(small * 2), "columns": np.where((i // 4) % 256 == 17, 10 + rng.random(V), small),
-           "blocks": np.where(i // 1024 == (V // 1024) // 2, 10 + small, small),
-           "threads over": np.where((i // 4) % 256 < K, 20 + small, np.minimum(small, 3)),
-           "tail": np.where(i >= V - K, 9.0 + i * 1e-5, small), "head": np.where(i < 3, 9.0, small)}[shape]
-    if shape == "threads over":  # all but one of K threads' columns hold larger values than its best
-        row = np.where((i // 4) % 256 == K - 1, 5.0 + 0.01 * small, row)
-    check(cuda_rt, np.stack([row, row[::-1], small]), [0, V - 1, V // 2], K)
+    row = pattern(shape, V, K, rng)
+    check(cuda_rt, np.stack([row, row[::-1], rng.standard_normal(V)]), [0, V - 1, V // 2], K)
+
+
+@pytest.mark.parametrize("R, V", [(2400, 1025), (2400, 2050), (2401, 4096), (2402, 8191), (900, 5000), (1000, 20001),
+                                  (10000, 258), (5000, 500)])
+@pytest.mark.parametrize("K", [0, 3, 8, 20, 32])
+def test_alternatives_of_many_rows(cuda_rt, R, V, K):
+    """The same patterns in batches, whose rows other teams of threads take:
+    warps for up to 8192 logits, CTAs of 128 threads, groups of lanes."""
+    rng = np.random.default_rng(R + V + K)
+    rows = [bf16(pattern(s, V, max(K, 1), rng)) for s in SHAPES + ["normal"] * 5]
+    mask = np.where(rng.random(V) < 0.97, -np.inf, rows[-1])
+    rows += [mask, np.full(V, -np.inf), np.where(np.arange(V) == V // 2, np.nan, rows[-1]),
+             np.where(np.arange(V) == V - 1, np.inf, rows[-1]), np.full(V, LOW)]
+    x = np.array(rows, np.float32)
+    n = len(x)
+    ids = rng.integers(-1, V, n)
+    big, all_ids = np.tile(x, (R // n + 1, 1))[:R], np.tile(ids, R // n + 1)[:R]
+    got, want = forward(cuda_rt, big, all_ids, K, kind=K % 2, pad=K % 3), logprobs(x, ids, K)
+    lp, ent = logprobs_tolerance(want, V)
+    tol = {"logp": lp(want["logp"]), "entropy": ent, "top_logp": lp(want["top_logp"])}
+    for r0 in range(0, R, n):
+        m = min(n, R - r0)
+        assert np.array_equal(got["top_ids"][r0:r0 + m], want["top_ids"][:m])
+        for k in tol:
+            near(got[k][r0:r0 + m], want[k][:m], tol[k][:m], k)
+
+
+def test_offsets_beyond_32_bits(cuda_rt):
+    """Rows 1.1 * 10^9 logits apart: the third starts past 2^31 values."""
+    rt = cuda_rt
+    ld, V = 1100000003, 3001
+    p = ctypes.c_void_p()
+    assert rt.lib.tp_alloc((2 * ld + V) * 4, ctypes.byref(p)) == 0
+    x = (np.random.default_rng(3).standard_normal((3, V)) * 3).astype(np.float32)
+    for r in range(3):
+        assert rt.lib.tp_memcpy_h2d(p.value + 4 * ld * r, x[r].ctypes.data_as(ctypes.c_void_p), 4 * V) == 0
+    I, L, S, E = (Buf(rt, a) for a in (np.array([5, 0, V - 1], np.int32), np.zeros(3, np.float32),
+                                       np.zeros((3, 2), np.float32), np.zeros(3, np.float32)))
+    T, TL, G = Buf(rt, np.zeros((3, 4), np.int32)), Buf(rt, np.zeros((3, 4), np.float32)), Buf(rt, np.ones(3, np.float32))
+    assert rt.lib.tpk_token_logprobs(p.value, ld, I.ptr, 1, 3, V, 4, L.ptr, E.ptr, S.ptr, T.ptr, TL.ptr) == 0
+    want = logprobs(x, [5, 0, V - 1], 4)
+    lp, _ = logprobs_tolerance(want, V)
+    near(L.read(), want["logp"], lp(want["logp"]), "logp")
+    assert np.array_equal(T.read(), want["top_ids"])
+    assert rt.lib.tpk_token_logprobs_backward(p.value, ld, I.ptr, 1, S.ptr, E.ptr, G.ptr, None, 3, V, p.value, ld) == 0
+    d, tol = logprobs_grad(x, [5, 0, V - 1], None, None, np.ones(3), None)
+    for r in range(3):
+        got = np.empty(V, np.float32)
+        assert rt.lib.tp_memcpy_d2h(got.ctypes.data_as(ctypes.c_void_p), p.value + 4 * ld * r, 4 * V) == 0
+        near(got, d[r], tol[r], "dlogits")
+    assert rt.lib.tp_free(p.value) == 0
 
 
 def test_many_rows(cuda_rt):
