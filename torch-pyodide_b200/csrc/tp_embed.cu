@@ -132,9 +132,10 @@ __global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dou
 // are n D 4 bytes from HBM.)
 constexpr int SORT_NT = 1024;
 constexpr int SORT_WARPS = SORT_NT / 32;
-constexpr int SORT_TOKENS = 512;          // tokens of one CTA, at most
-constexpr int SORT_WORDS = 16384;         // positions / 32 whose hits are kept in shared memory
-constexpr int SORT_U = 16;                // ids of a thread in flight
+constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a thread each in the scan)
+constexpr int SORT_WORDS = 8192;          // positions / 32 whose hits are kept in shared memory
+constexpr int SORT_LIST = 768;            // hits that a warp lists before it places them
+constexpr int SORT_U = 16;                // ids of a thread in flight, and words listed at once
 
 struct EmbedSort {
   int g;          // log2 of the CTAs
@@ -159,8 +160,8 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   __shared__ int32_t sh[SORT_WARPS];
   const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
   int32_t* count = sort_sm;                                  // [warps][W]
-  uint16_t* hits = (uint16_t*)(sort_sm + SORT_WARPS * W);    // [warps][1024]
-  uint32_t* words = (uint32_t*)(hits + SORT_WARPS * 1024);   // hits of 32 positions each
+  uint16_t* hits = (uint16_t*)(sort_sm + SORT_WARPS * W);    // [warps][SORT_LIST]
+  uint32_t* words = (uint32_t*)(hits + SORT_WARPS * SORT_LIST);   // hits of 32 positions each
   const int64_t nwords = (e.n + 31) >> 5;
   const bool kept = nwords <= SORT_WORDS;
   const int64_t per = (nwords + SORT_WARPS - 1) / SORT_WARPS;  // words of one warp: neighbours, so that order is kept
@@ -227,31 +228,37 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
     if (me == (int)gridDim.x - 1 && t == W - 1) e.start[(int64_t)gridDim.x * W] = first + c;
   }
   __syncthreads();
-  // 32 words at a time: a lane lists its word's hits, in order, as offsets from the
-  // first word's position; then the hits are placed 32 at a time, a lane each, the
-  // tokens of the next 32 under way.
-  uint16_t* list = hits + 1024 * w;
-  for (int64_t i = w0; i < w1; i += 32) {
+  // 16 words at a time, a lane lists its word's hits, in order, as offsets from the
+  // list's first word; a list that has grown long is placed, 32 hits at a time, a
+  // lane each, the tokens of the next 32 under way.
+  uint16_t* list = hits + SORT_LIST * w;
+  int have = 0;
+  int64_t list0 = w0;  // the word that offsets count from
+  for (int64_t i = w0; i < w1; i += SORT_U) {
     uint32_t mine = 0u;
     if (kept) {
-      if (i + lane < w1) mine = words[i + lane];
+      if (lane < SORT_U && i + lane < w1) mine = words[i + lane];
     } else {
-      for (int j = 0; j < 32; ++j) {
+      for (int j = 0; j < SORT_U; ++j) {
         const int v = token(i + j);
         const uint32_t b = __ballot_sync(0xffffffffu, e.valid(v) && e.owner(v) == me);
         if (lane == j) mine = b;
       }
     }
     int at = __popc(mine);
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, at, o);
       if (lane >= o) at += u;
     }
-    const int have = __shfl_sync(0xffffffffu, at, 31);
-    at -= __popc(mine);
-    for (; mine; mine &= mine - 1) list[at++] = (uint16_t)(32 * lane + __ffs(mine) - 1);
+    const int more = __shfl_sync(0xffffffffu, at, 31);
+    at += have - __popc(mine);
+    for (; mine; mine &= mine - 1) list[at++] = (uint16_t)(32 * (i - list0 + lane) + __ffs(mine) - 1);
+    have += more;
+    // room for 16 words more, offsets of them within 16 bits, or the end
+    if (have <= SORT_LIST - 32 * SORT_U && i + 2 * SORT_U - list0 <= 2048 && i + SORT_U < w1) continue;
     __syncwarp();
-    const int64_t first = i * 32;
+    const int64_t first = list0 * 32;
     auto fetch = [&](int h) { return h < have ? token_id(e.ids, KIND, first + list[h]) : 0; };
     int v = fetch(lane);
     for (int h = 0; h < have; h += 32) {
@@ -269,6 +276,8 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
       __syncwarp();
       v = next;
     }
+    have = 0;
+    list0 = i + SORT_U;
   }
 }
 
@@ -554,12 +563,12 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   e.pos = (int32_t*)(base + p.pos);
   e.tok = (int32_t*)(base + p.tok);
   const int64_t words = (n + 31) / 32;
-  const size_t smem = (size_t)(SORT_WARPS * p.per + SORT_WARPS * 512 + (words <= SORT_WORDS ? words : 0)) * 4;
+  const size_t smem = (size_t)(SORT_WARPS * (p.per + SORT_LIST / 2) + (words <= SORT_WORDS ? words : 0)) * 4;
   auto sort = kind == IDS_I32 ? k_embed_sort<IDS_I32> : k_embed_sort<IDS_F32>;
   static bool raised[2] = {false, false};
-  if (!raised[kind]) {  // 64 KB each of counts, listed hits and hits at most
+  if (!raised[kind]) {  // 128 KB of counts, 48 of listed hits, 32 of hits at most
     TP_CUDA(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (SORT_WARPS * (SORT_TOKENS + 512) + SORT_WORDS) * 4));
+                                 (SORT_WARPS * (SORT_TOKENS + SORT_LIST / 2) + SORT_WORDS) * 4));
     raised[kind] = true;
   }
   TP_LAUNCH(sort, 1u << p.g, SORT_NT, smem, e);
