@@ -97,7 +97,8 @@ struct LpRow {
 };
 
 // ---- short rows: a group of L lanes each, the row in registers --------------------------
-// Lane l of the group holds the logits l + L k, k < N.  Smaller groups spend
+// The row is read in 16-byte vectors from the boundary at or below its start:
+// lane l of the group holds the vectors l + L k, k < N.  Smaller groups spend
 // fewer instructions per row on exchanging (a warp works on 32 / L rows at
 // once), larger ones finish a single row sooner.  The alternatives (K <= L of
 // them): at least K logits are as large as the K-th largest of the lanes' maxima;
@@ -120,18 +121,29 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
   const float* __restrict__ xr = x + row * ld;
   int t = -1;
   if (logp && live && l == 0) t = token_id(ids, kind, row);
-  float v[N];
+  const int a = (int)(((uintptr_t)xr >> 2) & 3), end = live ? a + V : 0;  // the row is base[a .. end)
+  const float* __restrict__ base = xr - a;
+  float v[4 * N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = live && l + L * k < V ? xr[l + L * k] : -INFINITY;
+  for (int k = 0; k < N; ++k) {
+    const int u = 4 * (l + L * k);
+    if (u + 4 <= end && (k > 0 || u >= a)) {
+      const float4 q = *reinterpret_cast<const float4*>(base + u);
+      v[4 * k] = q.x, v[4 * k + 1] = q.y, v[4 * k + 2] = q.z, v[4 * k + 3] = q.w;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[4 * k + c] = u + c >= a && u + c < end ? base[u + c] : -INFINITY;
+    }
+  }
   const float xt = t >= 0 && t < V ? xr[t] : 0.0f;
   LpStat s{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < N; ++k) s.m = lp_max(s.m, v[k]);
+  for (int k = 0; k < 4 * N; ++k) s.m = lp_max(s.m, v[k]);
   float tau = s.m;
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(ALL, s.m, o));
 #pragma unroll
-  for (int k = 0; k < N; ++k) s.add(v[k]);
+  for (int k = 0; k < 4 * N; ++k) s.add(v[k]);
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) {
     s.S += __shfl_xor_sync(ALL, s.S, o);
@@ -140,6 +152,7 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
   const LpRow r(s);
   if (live && l == 0) r.write(s, row, V, t, xt, logp, entropy, stats);
   if constexpr (TOP) {
+    auto index = [&](int k) { return 4 * (l + L * (k >> 2)) + (k & 3) - a; };  // of v[k] in the row
 #pragma unroll
     for (int size = 2; size <= L; size <<= 1)  // the lanes' maxima in order, larger first
 #pragma unroll
@@ -151,15 +164,14 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
     unsigned long long some = 0ull;
     if (!r.bad) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) some |= v[k] >= tau ? 1ull << k : 0ull;
+      for (int k = 0; k < 4 * N; ++k) some |= v[k] >= tau ? 1ull << k : 0ull;
     }
     if (l == 0) cands[g] = 0;
     __syncwarp();
     while (some) {
-      const int k = __ffsll((long long)some) - 1;
+      const int i = index(__ffsll((long long)some) - 1), to = atomicAdd(&cands[g], 1);
       some &= some - 1;
-      const int i = atomicAdd(&cands[g], 1);
-      if (i < CAND) cand[g][i] = lp_key(xr[l + L * k], (uint32_t)(l + L * k));
+      if (to < CAND) cand[g][to] = lp_key(xr[i], (uint32_t)i);
     }
     __syncwarp();
     const int n = cands[g];
@@ -168,8 +180,8 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
       for (int q = 0; q < K; ++q) {
         unsigned long long best = 0ull;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const unsigned long long y = lp_key(v[k], (uint32_t)(l + L * k));
+        for (int k = 0; k < 4 * N; ++k) {
+          const unsigned long long y = lp_key(v[k], (uint32_t)index(k));
           if (v[k] > -INFINITY && y < last && y > best) best = y;
         }
 #pragma unroll
@@ -666,32 +678,61 @@ struct LpGrad {
   }
 };
 
-// Rows of at most 1024 logits: a warp each.
-__global__ void __launch_bounds__(256) k_logprobs_bwd_warp(const float* x, int64_t ld, const void* __restrict__ ids,
-                                                           int kind, const float* __restrict__ stats,
-                                                           const float* __restrict__ entropy,
-                                                           const float* __restrict__ dlogp,
-                                                           const float* __restrict__ dentropy, int64_t R, int V,
-                                                           float* dx, int64_t ldd) {
+// Rows of at most 1024 logits: a group of L lanes each, in 16-byte vectors where
+// the row of x and the row of dx start at the same offset from a boundary.
+template <int L>
+__global__ void __launch_bounds__(128) k_logprobs_bwd_short(const float* x, int64_t ld, const void* __restrict__ ids,
+                                                            int kind, const float* __restrict__ stats,
+                                                            const float* __restrict__ entropy,
+                                                            const float* __restrict__ dlogp,
+                                                            const float* __restrict__ dentropy, int64_t R, int V,
+                                                            float* dx, int64_t ldd) {
   ::tp::pdl_enter();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int l = threadIdx.x % L;
+  const int64_t row = (int64_t)blockIdx.x * (128 / L) + threadIdx.x / L;
   if (row >= R) return;
   const float* xr = x + row * ld;
   float* dr = dx + row * ldd;
-  float v[8];
-  auto load = [&](int i) {
+  const int a = (int)(((uintptr_t)xr >> 2) & 3);
+  if ((((uintptr_t)dr >> 2) & 3) == a) {
+    const int end = a + V;  // the row is base[a .. end)
+    const float* xb = xr - a;
+    float* db = dr - a;
+    float4 v[4];
+    auto whole = [&](int u) { return u >= a && u + 4 <= end; };
+    auto load = [&](int j) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + 32 * k < V) v[k] = xr[i + 32 * k];
-  };
-  load(lane);  // under way while the row's coefficients are fetched
-  const LpGrad g(row, V, ids, kind, stats, entropy, dlogp, dentropy);
-  for (int i = lane; i < V; i += 256) {
-    if (i > lane) load(i);
+      for (int q = 0; q < 4; ++q)
+        if (whole(4 * (j + L * q))) v[q] = *reinterpret_cast<const float4*>(xb + 4 * (j + L * q));
+    };
+    load(l);  // under way while the row's coefficients are fetched
+    const LpGrad g(row, V, ids, kind, stats, entropy, dlogp, dentropy);
+    for (int j = l; 4 * j < end; j += 4 * L) {
+      if (j > l) load(j);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + 32 * k < V) dr[i + 32 * k] = g.zero ? 0.0f : g(v[k], i + 32 * k);
+      for (int q = 0; q < 4; ++q) {
+        const int u = 4 * (j + L * q), i = u - a;
+        if (whole(u)) {
+          *reinterpret_cast<float4*>(db + u) =
+              g.zero ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                     : make_float4(g(v[q].x, i), g(v[q].y, i + 1), g(v[q].z, i + 2), g(v[q].w, i + 3));
+        } else {
+          for (int c = 0; c < 4; ++c)
+            if (u + c >= a && u + c < end) db[u + c] = g.zero ? 0.0f : g(xb[u + c], i + c);
+        }
+      }
+    }
+  } else {
+    const LpGrad g(row, V, ids, kind, stats, entropy, dlogp, dentropy);
+    for (int i = l; i < V; i += 8 * L) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + L * k < V) v[k] = xr[i + L * k];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + L * k < V) dr[i + L * k] = g.zero ? 0.0f : g(v[k], i + L * k);
+    }
   }
 }
 
@@ -754,26 +795,28 @@ __global__ void __launch_bounds__(LP_BWD_NT, 2048 / LP_BWD_NT) k_logprobs_bwd(co
 
 // Rows up to this long are held in registers.
 constexpr int64_t LP_SHORT = 1024;
+// Rows up to this long are 8 lanes' in the gradient, if there are many.
+constexpr int64_t LP_BWD_8 = 300;
 
 template <int L, bool TOP>
 static void launch_logprobs_short(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int V, int K,
                                   float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp) {
   const unsigned grid = (unsigned)((R + 128 / L - 1) / (128 / L));
 #define TP_LP_SHORT(N)                                                                                             \
-  if (V <= L * N) {                                                                                                \
+  if (V + 3 <= 4 * L * N) { /* a row may start 3 logits past a boundary */                                         \
     TP_LAUNCH((k_logprobs_short<L, N, TOP>), grid, 128, 0, x, ld, ids, kind, R, V, K, logp, entropy, stats, top_ids, \
               top_logp);                                                                                           \
     return;                                                                                                        \
   }
+  TP_LP_SHORT(1)
   TP_LP_SHORT(2)
+  TP_LP_SHORT(3)
   TP_LP_SHORT(4)
+  TP_LP_SHORT(5)
+  TP_LP_SHORT(6)
+  TP_LP_SHORT(7)
   TP_LP_SHORT(8)
-  TP_LP_SHORT(12)
-  TP_LP_SHORT(16)
-  TP_LP_SHORT(20)
-  TP_LP_SHORT(24)
-  TP_LP_SHORT(28)
-  TP_LP_SHORT(33)
+  TP_LP_SHORT(9)
 #undef TP_LP_SHORT
 }
 
@@ -818,7 +861,8 @@ void launch_logprobs(const float* x, int64_t ld, const void* ids, int kind, int6
   if (V <= LP_SHORT) {
     // the smallest group whose lanes hold the row and whose warps still fill the SMs
     const int64_t warps = (int64_t)sm_count() * 16;
-    const int L = V <= 8 * 33 && K <= 8 && R >= 4 * warps ? 8 : (V <= 16 * 33 && K <= 16 && R >= 2 * warps ? 16 : 32);
+    const int L = V <= 8 * 36 - 3 && K <= 8 && R >= 4 * warps ? 8
+                  : (V <= 16 * 36 - 3 && K <= 16 && R >= 2 * warps ? 16 : 32);
 #define TP_LP_GROUP(L)                                                                                                \
   if (K) launch_logprobs_short<L, true>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);   \
   else launch_logprobs_short<L, false>(x, ld, ids, kind, R, (int)V, K, logp, entropy, stats, top_ids, top_logp);
@@ -858,8 +902,12 @@ void launch_logprobs_bwd(const float* x, int64_t ld, const void* ids, int kind, 
                          float* dx, int64_t ldd) {
   if (R == 0) return;
   if (V <= LP_SHORT) {
-    TP_LAUNCH(k_logprobs_bwd_warp, (unsigned)((R + 7) / 8), 256, 0, x, ld, ids, kind, stats, entropy, dlogp, dentropy,
-              R, (int)V, dx, ldd);
+#define TP_LP_BWD(L)                                                                                                 \
+  TP_LAUNCH(k_logprobs_bwd_short<L>, (unsigned)((R + 128 / L - 1) / (128 / L)), 128, 0, x, ld, ids, kind, stats, entropy, \
+            dlogp, dentropy, R, (int)V, dx, ldd)
+    if (V <= LP_BWD_8 && R >= (int64_t)sm_count() * 64) TP_LP_BWD(8);
+    else TP_LP_BWD(32);
+#undef TP_LP_BWD
     return;
   }
   const int chunks = (int)((V + 3 + 16 * LP_BWD_NT - 1) / (16 * LP_BWD_NT));  // a row may start 3 logits past a boundary
