@@ -144,13 +144,13 @@ class Step:
                                    self.E, self.W, *self.m, *self.v)]
 
 
-@pytest.mark.parametrize("n", [140, 700])
-def test_captured_step_replays_on_new_inputs(cuda_rt, n):
+@pytest.mark.parametrize("n, V", [(140, 97), (700, 97), (24, 9001), (2500, 1500)])
+def test_captured_step_replays_on_new_inputs(cuda_rt, n, V):
     """A captured step, replayed on inputs written between, gives the bits of
     the same calls made one by one; replays need nothing cleared between."""
     rt = cuda_rt
-    E, W, *_ = make(n=n)
-    batches = [make(n=n, seed=s)[2:] for s in range(1, 5)]
+    E, W, *_ = make(V=V, n=n)
+    batches = [make(V=V, n=n, seed=s)[2:] for s in range(1, 5)]
     eager, graph = Step(rt, E, W, n), Step(rt, E, W, n)
     for s in (eager, graph):  # scratch of the linear layers reaches its size
         s.feed(*batches[0])

@@ -52,19 +52,19 @@ def test_logprobs_backward(lib, change, word):
     refused(lib, lib.tpk_token_logprobs_backward(*{**BACKWARD, **change}.values()), word)
 
 
-EMBED = dict(table=P, ld=8, ids=P, kind=0, n=5, vocab=10, dim=8, scale=1.0, out=P, ldo=8)
+EMBED = dict(table=P, ld=8, ids=P, kind=0, n=5, vocab=10, dim=8, scale=1.0, out=2 * P, ldo=8)
 
 
 @pytest.mark.parametrize("change, word", [
     (dict(n=-1), "tokens"), (dict(n=2 ** 31 - 1), "tokens"), (dict(vocab=0), "vocabulary"),
     (dict(vocab=2 ** 24 + 1), "vocabulary"), (dict(dim=-1), "width"), (dict(dim=2 ** 31, ld=2 ** 31, ldo=2 ** 31), "width"),
     (dict(ld=7), "row stride"), (dict(ldo=7), "row stride"), (dict(kind=2), "ids_kind"), (dict(table=None), "NULL"),
-    (dict(ids=None), "NULL"), (dict(out=None), "NULL"), (dict(out=P + 1), "aligned")])
+    (dict(ids=None), "NULL"), (dict(out=None), "NULL"), (dict(out=P + 1), "aligned"), (dict(out=P), "input")])
 def test_embedding(lib, change, word):
     refused(lib, lib.tpk_token_embedding(*{**EMBED, **change}.values()), word)
 
 
-GRAD = dict(dout=P, ldo=8, ids=P, kind=0, n=5, vocab=10, dim=8, scale=1.0, pad=-1, accumulate=0, dtable=P, ld=8, ws=P,
+GRAD = dict(dout=P, ldo=8, ids=P, kind=0, n=5, vocab=10, dim=8, scale=1.0, pad=-1, accumulate=0, dtable=2 * P, ld=8, ws=P,
             ws_bytes=1 << 20)
 
 
@@ -73,7 +73,8 @@ GRAD = dict(dout=P, ldo=8, ids=P, kind=0, n=5, vocab=10, dim=8, scale=1.0, pad=-
     (dict(ldo=7), "row stride"), (dict(kind=2), "ids_kind"), (dict(pad=-2), "padding_id"), (dict(pad=10), "padding_id"),
     (dict(accumulate=2), "accumulate"), (dict(dout=None), "NULL"), (dict(ids=None), "NULL"),
     (dict(dtable=None), "NULL"), (dict(ws_bytes=-1), "workspace"), (dict(n=5000, ws_bytes=8), "workspace"),
-    (dict(n=5000, ws=None), "workspace"), (dict(ws=P + 4), "workspace"), (dict(dtable=P + 2), "aligned")])
+    (dict(n=5000, ws=None), "workspace"), (dict(ws=P + 4), "workspace"), (dict(dtable=P + 2), "aligned"),
+    (dict(dtable=P), "input")])
 def test_embedding_backward(lib, change, word):
     refused(lib, lib.tpk_token_embedding_backward(*{**GRAD, **change}.values()), word)
 

@@ -46,6 +46,9 @@ static int block_cols(int64_t cols) {
 }
 
 // ---- lookup ---------------------------------------------------------------------------
+// A CTA per 512 columns of a row (or several narrow rows): the id, then the row,
+// are fetched one after the other, so it takes many CTAs to keep HBM busy.
+// 32768 x 2048: 59.5 us, 6.0 TB/s read and written.
 constexpr int EMB_U = 4;  // columns per thread, loaded before the first is stored
 
 template <int VEC>
@@ -286,7 +289,8 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
 // most 2 T goes whole to the tile it starts in.  A longer one is cut at the
 // tiles' borders: what came in from the tile before is the tile's partial 0, the
 // start of what goes on its partial 1 (what does both, partial 0).  T is 64, or
-// 16 where 64 would leave SMs without a tile.
+// 16 where 64 would leave SMs without a tile (65536 x 1024: 104 us with 64, 141 with
+// 16).  16384 x 4096 into 32000 rows written whole: 119 us, 6.6 TB/s.
 struct EmbedSum {
   const float* dout;
   int64_t ldo, cols;
@@ -435,7 +439,8 @@ __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(c
 
 // The runs that were cut: the tile one starts in adds up its partial 1 and the
 // partials 0 of the tiles after it, in f64: eight threads take every eighth,
-// and their sums are added in order.  A CTA looks through 8 tiles for such starts.
+// and their sums are added in order.  A CTA looks through 8 tiles for such starts
+// (16384 x 4096: 7 us; through 32: 11).
 constexpr int JOIN_TILES = 8, JOIN_ROWS = 8;
 
 template <bool ACC>
@@ -613,6 +618,7 @@ TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, 
     TP_REQUIRE(table && ids && out, "%s: table, ids and out must not be NULL", what);
     TP_REQUIRE((((uintptr_t)table | (uintptr_t)ids | (uintptr_t)out) & 3) == 0, "%s: a buffer is not 4-byte aligned",
                what);
+    TP_REQUIRE(out != table && (const void*)out != ids, "%s: out is an input", what);
     launch_embed(table, ld, ids, ids_kind, n, vocab, dim, scale, out, ldo);
   });
 }
@@ -639,6 +645,7 @@ TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const vo
     TP_REQUIRE(dtable && (n == 0 || (dout && ids)), "%s: dout, ids and dtable must not be NULL", what);
     TP_REQUIRE((((uintptr_t)dout | (uintptr_t)ids | (uintptr_t)dtable) & 3) == 0,
                "%s: a buffer is not 4-byte aligned", what);
+    TP_REQUIRE(dtable != dout && (const void*)dtable != ids, "%s: dtable is an input", what);
     const int64_t need = embed_bwd_ws(n, vocab, dim);
     TP_REQUIRE(ws_bytes >= need && (need == 0 || ws), "%s: a workspace of %lld bytes, %lld are needed", what,
                (long long)ws_bytes, (long long)need);
