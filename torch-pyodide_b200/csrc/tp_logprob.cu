@@ -27,6 +27,7 @@
 namespace tp {
 
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_MAX_PARTS = 8;  // CTAs of a cluster
 
 // Order of the alternatives: larger logit first, then the lower index; one
 // 64-bit key, larger is better.  Adding 0 makes -0 and 0 the same logit.
@@ -278,15 +279,21 @@ template <int NT>
 struct LpShared {
   static constexpr int CAND = NT == 32 ? 256 : 512;  // collected logits
   static constexpr int LIST = NT == 32 ? 128 : 256;  // units read again
-  LpStat warp[NT / 32], part;          // part: read by the cluster's first CTA
+  LpStat warp[NT / 32];
   float kth[NT / 32];                  // per warp: a value that K / (NT / 32) of its threads' maxima reach
-  unsigned long long top[LP_MAX_TOP];  // the part's alternatives, read by the first CTA too
+  unsigned long long top[LP_MAX_TOP];  // the part's alternatives
   unsigned short chosen[LIST];         // the units read again: 4 thread + vector
   float value[LIST], tau;              // and their maxima; the K-th largest of these
   unsigned short owner[NT];            // ties: threads
   unsigned long long cand[CAND];
   unsigned long long k[NT / 32], least;
   int units, cands;
+};
+
+// Where the cluster's CTAs leave what their parts came to: in the first one.
+struct LpGather {
+  LpStat part[LP_MAX_PARTS];
+  unsigned long long top[LP_MAX_PARTS * LP_MAX_TOP];
 };
 
 template <int NT>
@@ -492,28 +499,25 @@ __device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int 
   }
 }
 
-__device__ __forceinline__ uint32_t lp_peer(const void* p, int rank) {
+// p's place in the cluster's first CTA
+__device__ __forceinline__ uint32_t lp_first(const void* p) {
   uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)));
   return r;
 }
-__device__ __forceinline__ void lp_cluster_sync() {
-  asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+__device__ __forceinline__ void lp_put(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
 }
-__device__ __forceinline__ float lp_peer_f32(uint32_t at) {
-  float f;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(at) : "memory");
-  return f;
-}
-__device__ __forceinline__ unsigned long long lp_peer_u64(uint32_t at) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
-  return v;
+__device__ __forceinline__ void lp_put(uint32_t at, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 
-// NT: threads of a team (a warp: four teams to a CTA); parts: CTAs per row, the
-// cluster's size
-template <int NT, bool TOP>
+// NT: threads of a team (a warp: four teams to a CTA); SPLIT: a row is a cluster's,
+// of `parts` CTAs.  Few CTAs have the SMs to themselves then, so each fetches its
+// next batch ahead (64 x 131072 with 20 alternatives: 16.5 us, 18.2 without; with every
+// SM full the registers for it cost more than it brings, 619 us against 590 for
+// 8192 x 131072).
+template <int NT, bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
     k_logprobs_long(const float* __restrict__ x, int64_t ld, const void* __restrict__ ids, int kind, int64_t R,
                     int64_t V, int parts, int K, float* __restrict__ logp, float* __restrict__ entropy,
@@ -521,6 +525,9 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
   ::tp::pdl_enter();
   constexpr int TEAMS = NT == 32 ? 4 : 1, WARPS = NT / 32;
   __shared__ LpShared<NT> shared[TEAMS];
+  __shared__ LpGather all;
+  // the first CTA has to be there before another writes to it: asked here, waited for below
+  if (SPLIT) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   LpShared<NT>& sh = shared[threadIdx.x / NT];
   const int t = threadIdx.x % NT, lane = t & 31;
   int64_t row;
@@ -528,9 +535,11 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
   if (NT == 32) {
     row = (int64_t)blockIdx.x * TEAMS + threadIdx.x / NT;
     if (row >= R) return;
-  } else {
+  } else if (SPLIT) {
     row = blockIdx.x / parts;
     part = (int)(blockIdx.x - row * parts);
+  } else {
+    row = blockIdx.x;
   }
   const float* __restrict__ xr = x + row * ld;
   int tok = -1;
@@ -539,16 +548,24 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
     tok = token_id(ids, kind, row);
     if (tok >= 0 && tok < V) xt = xr[tok];
   }
-  const int64_t per = (V + parts - 1) / parts;
+  const int64_t per = SPLIT ? (V + parts - 1) / parts : V;
   const int64_t lo = per * part < V ? per * part : V, hi = lo + per < V ? lo + per : V;
   const LpPart<NT> p(xr, lo, hi);
   const int batches = p.batches();
   LpStat s{-INFINITY, 0.0f, 0.0f};
   float um[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   int mb = 0;
+  float4 next[SPLIT ? 4 : 1];
+  if constexpr (SPLIT) p.batch(0, t, next);
   for (int b = 0; b < batches; ++b) {
     float4 v[4];
-    p.batch(b, t, v);
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = next[q];
+      if (b + 1 < batches) p.batch(b + 1, t, next);
+    } else {
+      p.batch(b, t, v);
+    }
     float m;
     if (TOP) {
 #pragma unroll
@@ -625,43 +642,41 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
     if (s.m < INFINITY) lp_select<NT>(t, p, um, mb, tau, K, sh);  // not with a NaN or +inf in the part
     lp_sync<NT>();
   }
-  if (NT != 32 && parts > 1) {
-    if (t == 0) sh.part = s;
-    lp_cluster_sync();
-    if (part == 0) {
-      float m = s.m;
-      for (int c = 1; c < parts; ++c) m = lp_max(m, lp_peer_f32(lp_peer(&sh.part.m, c)));
-      LpStat all{s.m, s.S, s.T};
-      all.move(m);
-      for (int c = 1; c < parts; ++c) {
-        LpStat o{lp_peer_f32(lp_peer(&sh.part.m, c)), lp_peer_f32(lp_peer(&sh.part.S, c)),
-                 lp_peer_f32(lp_peer(&sh.part.T, c))};
-        o.move(m);
-        all.S += o.S;
-        all.T += o.T;
-      }
-      s = all;
-      if (TOP && m < INFINITY) {
-        // the parts' lists (0-padded) side by side, then the best of them
-        const int n = parts * K;
-        for (int i = t; i < n; i += NT) {
-          const int c = i / K;
-          sh.cand[i] = lp_peer_u64(lp_peer(&sh.top[i - c * K], c));
-        }
-        __syncthreads();
-        if (t < K) sh.top[t] = 0ull;
-        __syncthreads();
-        for (int i = t; i < n; i += NT) {
-          const unsigned long long k = sh.cand[i];
-          int r = 0;
-          for (int j = 0; j < n; ++j) r += sh.cand[j] > k;
-          if (r < K && k) sh.top[r] = k;
-        }
-        __syncthreads();
-      }
+  if (SPLIT) {
+    asm volatile("barrier.cluster.wait;" ::: "memory");
+    if (t == 0) {
+      const uint32_t at = lp_first(&all.part[part]);
+      lp_put(at, s.m);
+      lp_put(at + 4, s.S);
+      lp_put(at + 8, s.T);
     }
-    lp_cluster_sync();
+    if (TOP && t < K) lp_put(lp_first(&all.top[part * K + t]), sh.top[t]);
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
     if (part != 0) return;
+    s = all.part[0];
+    float m = s.m;
+    for (int c = 1; c < parts; ++c) m = lp_max(m, all.part[c].m);
+    s.move(m);
+    for (int c = 1; c < parts; ++c) {
+      LpStat o = all.part[c];
+      o.move(m);
+      s.S += o.S;
+      s.T += o.T;
+    }
+    if (TOP && m < INFINITY) {
+      // the parts' lists (0-padded) side by side, then the best of them
+      const int n = parts * K;
+      if (t < K) sh.top[t] = 0ull;
+      __syncthreads();
+      if (t < n) {
+        const unsigned long long k = all.top[t];
+        int r = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) r += all.top[j] > k;
+        if (r < K && k) sh.top[r] = k;
+      }
+      __syncthreads();
+    }
   }
   if (t >= 32) return;
   const LpRow r(s);
@@ -895,21 +910,20 @@ void launch_logprobs(const float* x, int64_t ld, const void* ids, int kind, int6
   const int nt = lp_threads(R, V);
   // more CTAs per row while the rows alone leave SMs empty and a part keeps half a batch
   int parts = 1;
-  while (nt == 256 && parts < 8 && R * parts < 4 * (int64_t)sm_count() && V / (2 * parts) >= 2048) parts *= 2;
+  while (nt == 256 && parts < LP_MAX_PARTS && R * parts < 4 * (int64_t)sm_count() && V / (2 * parts) >= 2048) parts *= 2;
   const int64_t ctas = nt == 32 ? (R + 3) / 4 : R * parts;
   TP_REQUIRE(ctas <= INT_MAX, "token_logprobs: %lld rows are too many", (long long)R);
-#define TP_LP_LONG(NT)                                                                                                 \
-  if (nt == NT) {                                                                                                      \
-    if (K)                                                                                                             \
-      launch_cluster(k_logprobs_long<NT, true>, (unsigned)ctas, NT == 32 ? 128 : NT, parts, x, ld, ids, kind, R, V, parts, \
-                     K, logp, entropy, stats, top_ids, top_logp);                                                      \
-    else                                                                                                               \
-      launch_cluster(k_logprobs_long<NT, false>, (unsigned)ctas, NT == 32 ? 128 : NT, parts, x, ld, ids, kind, R, V, parts, \
-                     K, logp, entropy, stats, top_ids, top_logp);                                                      \
-  }
-  TP_LP_LONG(32)
-  TP_LP_LONG(128)
-  TP_LP_LONG(256)
+#define TP_LP_LONG(NT, TOP, SPLIT)                                                                                  \
+  launch_cluster(k_logprobs_long<NT, TOP, SPLIT>, (unsigned)ctas, NT == 32 ? 128 : NT, parts, x, ld, ids, kind, R, V, \
+                 parts, K, logp, entropy, stats, top_ids, top_logp)
+  if (nt == 32 && K) TP_LP_LONG(32, true, false);
+  else if (nt == 32) TP_LP_LONG(32, false, false);
+  else if (nt == 128 && K) TP_LP_LONG(128, true, false);
+  else if (nt == 128) TP_LP_LONG(128, false, false);
+  else if (parts > 1 && K) TP_LP_LONG(256, true, true);
+  else if (parts > 1) TP_LP_LONG(256, false, true);
+  else if (K) TP_LP_LONG(256, true, false);
+  else TP_LP_LONG(256, false, false);
 #undef TP_LP_LONG
 }
 
