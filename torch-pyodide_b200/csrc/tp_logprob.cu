@@ -187,10 +187,9 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
       unsigned long long last = ~0ull;
       for (int q = 0; q < K; ++q) {
         unsigned long long best = 0ull;
-#pragma unroll
-        for (int k = 0; k < 4 * N; ++k) {
-          const unsigned long long y = lp_key(v[k], (uint32_t)index(k));
-          if (v[k] > -INFINITY && y < last && y > best) best = y;
+        for (int i = l; live && i < V; i += L) {  // from L1 or L2: registers for this would cost every row
+          const unsigned long long y = lp_key(xr[i], (uint32_t)i);
+          if (xr[i] > -INFINITY && y < last && y > best) best = y;
         }
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) {
