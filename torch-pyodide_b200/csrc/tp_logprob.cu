@@ -241,6 +241,7 @@ struct LpPart {
   const float* base;  // the boundary at or below the part's first logit
   int a, end;         // its logits are base[a .. end)
   int64_t lo;         // the row index of base[0] (negative below the row's start)
+  LpPart() = default;
   __device__ LpPart(const float* xr, int64_t lo_, int64_t hi) {
     const float* p = xr + lo_;
     a = (int)(((uintptr_t)p >> 2) & 3);
@@ -366,6 +367,86 @@ __device__ __forceinline__ void lp_reread(int t, const LpPart<NT>& p, const unsi
   }
 }
 
+template <int NT>
+__device__ __forceinline__ void lp_add(LpShared<NT>& sh, float x, uint32_t at) {
+  const int i = atomicAdd(&sh.cands, 1);
+  if (i < LpShared<NT>::CAND) sh.cand[i] = lp_key(x, at);
+}
+
+// lp_select where ties overflow a list: threads in the place of units.  m: this
+// thread's maximum if it is one of those that reach tau, else -inf.  Not inlined:
+// what it needs in registers is not held through the walk.
+template <int NT>
+__device__ __noinline__ void lp_select_ties(int t, const float* base, int a, int end, int64_t lo, float m, int mb,
+                                            int K, LpShared<NT>& sh) {
+  LpPart<NT> p;
+  p.base = base;
+  p.a = a;
+  p.end = end;
+  p.lo = lo;
+  lp_sync<NT>();
+  if (t == 0) sh.units = sh.cands = 0, sh.least = 0ull;
+  lp_sync<NT>();
+  if (m > -INFINITY) {
+    float4 x[4];
+    p.batch(mb, t, x);
+    int at = 0;
+#pragma unroll
+    for (int q = 3; q >= 0; --q) {
+      const int u = 4 * (mb * 4 * NT + q * NT + t);
+      if (x[q].w == m) at = u + 3;
+      if (x[q].z == m) at = u + 2;
+      if (x[q].y == m) at = u + 1;
+      if (x[q].x == m) at = u;
+    }
+    const int i = atomicAdd(&sh.units, 1);
+    sh.cand[i] = lp_key(m, (uint32_t)(p.lo + at));
+    sh.owner[i] = (unsigned short)t;
+  }
+  lp_sync<NT>();
+  const int n = sh.units;
+  const int chosen = 4 * (n < K ? n : K);
+  for (int u = t; u < n; u += NT) {
+    const unsigned long long k = sh.cand[u];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
+    if (above < K)
+      for (int q = 0; q < 4; ++q) sh.chosen[4 * above + q] = (unsigned short)(4 * sh.owner[u] + q);
+    if (above == K - 1) sh.least = k;
+  }
+  lp_sync<NT>();
+  const unsigned long long least = sh.least;
+  lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
+    if (x > -INFINITY && lp_key(x, at) >= least) lp_add(sh, x, at);
+  });
+  lp_sync<NT>();
+  const int nc = sh.cands;
+  if (nc <= LpShared<NT>::CAND) {
+    lp_rank<NT>(t, sh.cand, nc, K, sh.top);
+    return;
+  }
+  // More than the list holds (a few threads with most of the row's large values):
+  // one alternative after the other, the best that is worse than the one before.
+  unsigned long long last = ~0ull;
+  for (int q = 0; q < K; ++q) {
+    unsigned long long best = 0ull;
+    lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
+      const unsigned long long k = lp_key(x, at);
+      if (x > -INFINITY && k < last && k > best) best = k;
+    });
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
+      best = u > best ? u : best;
+    }
+    if ((t & 31) == 0) sh.k[t >> 5] = best;
+    lp_sync<NT>();
+    for (int i = 0; i < NT / 32; ++i) best = sh.k[i] > best ? sh.k[i] : best;
+    if (t == 0) sh.top[q] = best;
+    last = best;
+    lp_sync<NT>();
+  }
+}
+
 // The K best keys of the part into sh.top, by thread t of the team.  um: this
 // thread's unit maxima, mb: the batch its largest came from first, tau: a value
 // that at least K units reach; the counters are 0.
@@ -418,13 +499,9 @@ __device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int 
     lp_sync<NT>();
     n = sh.units;
   }
-  auto add = [&](float x, uint32_t at) {
-    const int i = atomicAdd(&sh.cands, 1);
-    if (i < LpShared<NT>::CAND) sh.cand[i] = lp_key(x, at);
-  };
   if (n <= LpShared<NT>::LIST) {
     lp_reread<NT>(t, p, sh.chosen, n, [&](float x, uint32_t at) {
-      if (x >= tau) add(x, at);
+      if (x >= tau) lp_add(sh, x, at);
     });
     lp_sync<NT>();
     const int nc = sh.cands;
@@ -433,69 +510,7 @@ __device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int 
       return;
     }
   }
-  // Ties: threads in the place of units, and where in its batch the maximum of each stands.
-  lp_sync<NT>();
-  if (t == 0) sh.units = sh.cands = 0, sh.least = 0ull;
-  lp_sync<NT>();
-  if (in) {
-    const float m = fmaxf(fmaxf(um[0], um[1]), fmaxf(um[2], um[3]));
-    float4 x[4];
-    p.batch(mb, t, x);
-    int at = 0;
-#pragma unroll
-    for (int q = 3; q >= 0; --q) {
-      const int u = 4 * (mb * 4 * NT + q * NT + t);
-      if (x[q].w == m) at = u + 3;
-      if (x[q].z == m) at = u + 2;
-      if (x[q].y == m) at = u + 1;
-      if (x[q].x == m) at = u;
-    }
-    const int i = atomicAdd(&sh.units, 1);
-    sh.cand[i] = lp_key(m, (uint32_t)(p.lo + at));
-    sh.owner[i] = (unsigned short)t;
-  }
-  lp_sync<NT>();
-  n = sh.units;
-  const int chosen = 4 * (n < K ? n : K);
-  for (int u = t; u < n; u += NT) {
-    const unsigned long long k = sh.cand[u];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
-    if (above < K)
-      for (int q = 0; q < 4; ++q) sh.chosen[4 * above + q] = (unsigned short)(4 * sh.owner[u] + q);
-    if (above == K - 1) sh.least = k;
-  }
-  lp_sync<NT>();
-  const unsigned long long least = sh.least;
-  lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
-    if (x > -INFINITY && lp_key(x, at) >= least) add(x, at);
-  });
-  lp_sync<NT>();
-  const int nc = sh.cands;
-  if (nc <= LpShared<NT>::CAND) {
-    lp_rank<NT>(t, sh.cand, nc, K, sh.top);
-    return;
-  }
-  // More than the list holds (a few threads with most of the row's large values):
-  // one alternative after the other, the best that is worse than the one before.
-  unsigned long long last = ~0ull;
-  for (int q = 0; q < K; ++q) {
-    unsigned long long best = 0ull;
-    lp_reread<NT>(t, p, sh.chosen, chosen, [&](float x, uint32_t at) {
-      const unsigned long long k = lp_key(x, at);
-      if (x > -INFINITY && k < last && k > best) best = k;
-    });
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long u = __shfl_xor_sync(0xffffffffu, best, o);
-      best = u > best ? u : best;
-    }
-    if ((t & 31) == 0) sh.k[t >> 5] = best;
-    lp_sync<NT>();
-    for (int i = 0; i < NT / 32; ++i) best = sh.k[i] > best ? sh.k[i] : best;
-    if (t == 0) sh.top[q] = best;
-    last = best;
-    lp_sync<NT>();
-  }
+  lp_select_ties<NT>(t, p.base, p.a, p.end, p.lo, in ? fmaxf(fmaxf(um[0], um[1]), fmaxf(um[2], um[3])) : -INFINITY, mb, K, sh);
 }
 
 // p's place in the cluster's first CTA
