@@ -131,13 +131,17 @@ def test_gradient_of_long_sums(cuda_rt):
     check_grad(cuda_rt, rng.standard_normal((n, 3)), ids, 500, 0.5, old=rng.standard_normal((500, 3)).astype(np.float32))
 
 
+@pytest.mark.parametrize("n, V", [(600001, 3000), (40000, 1), (33000, 131072), (32769, 140000), (5000, 1000000),
+                                  (300001, 2 ** 20 + 5), (20000, 2 ** 20 + 5)])
 @pytest.mark.parametrize("accumulate", [False, True])
-def test_gradient_of_many_tokens(cuda_rt, accumulate):
-    """More positions than the sort keeps hits of in shared memory."""
+def test_gradient_of_many_tokens(cuda_rt, n, V, accumulate):
+    """Ids that are split by owner before they are sorted, and more positions than
+    one sort keeps hits of in shared memory."""
     rng = np.random.default_rng(17)
-    n, V = 600001, 3000
     old = rng.standard_normal((V, 2)).astype(np.float32) if accumulate else None
-    check_grad(cuda_rt, rng.standard_normal((n, 2)), zipf(rng, n, V), V, 1.0, pad=7, old=old)
+    ids = zipf(rng, n, V)
+    ids[::9] = -1
+    check_grad(cuda_rt, rng.standard_normal((n, 2)), ids, V, 1.0, pad=min(7, V) - 1, old=old, kind=n % 2)
 
 
 @pytest.mark.parametrize("V", [1, 149, 100000, 2 ** 20])

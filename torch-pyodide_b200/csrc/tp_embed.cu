@@ -138,6 +138,7 @@ constexpr int SORT_WARPS = SORT_NT / 32;
 constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a thread each in the scan)
 constexpr int SORT_WORDS = 8192;          // positions / 32 whose hits are kept in shared memory
 constexpr int SORT_LIST = 768;            // hits that a warp lists before it places them
+constexpr int SPLIT_G = 10;               // log2 of the owners that ids can be split by first
 constexpr int SORT_U = 16;                // ids of a thread in flight, and words listed at once
 
 struct EmbedSort {
@@ -155,6 +156,50 @@ struct EmbedSort {
   __device__ __forceinline__ int key(int v) const { return owner(v) * per + local(v); }
   __device__ __forceinline__ int total() const { return start[(int64_t)per << g]; }
 };
+
+// The counts [warps][W] of CTA `me`'s tokens become the places of each warp's
+// positions, those of its first token starting at `base`; start[] is written.
+__device__ __forceinline__ void embed_places(const EmbedSort& e, int32_t* count, int me, int base, int32_t* sh) {
+  const int W = e.per, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  int k[SORT_WARPS], c = 0;  // one thread per token
+  if (t < W)
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) k[i] = count[i * W + t];
+  if (t < W)
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) c += k[i];
+  int incl = c;  // scan over the tokens
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) sh[w] = incl;
+  __syncthreads();
+  int first = base + incl - c;
+  for (int i = 0; i < w; ++i) first += sh[i];
+  if (t < W) {
+    e.start[(int64_t)me * W + t] = first;
+    int at = first;
+#pragma unroll
+    for (int i = 0; i < SORT_WARPS; ++i) {
+      count[i * W + t] = at;
+      at += k[i];
+    }
+    if (me == (1 << e.g) - 1 && t == W - 1) e.start[(int64_t)W << e.g] = first + c;
+  }
+  __syncthreads();
+}
+
+// Where this lane's key stands: its place among the lanes of `some` (the ones that
+// call) with the same key, after the key's counter, which moves on by their number.
+__device__ __forceinline__ int embed_take(uint32_t some, int key, int32_t* counter) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t peers = __match_any_sync(some, key);
+  const int rank = __popc(peers & ((1u << lane) - 1)), to = *counter;
+  __syncwarp(some);
+  if (rank == 0) *counter = to + __popc(peers);
+  return to + rank;
+}
 
 template <int KIND>
 __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
@@ -203,34 +248,7 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   int base = 0;
   for (int i = 0; i < SORT_WARPS; ++i) base += sh[i];
   __syncthreads();
-  // one thread per token: its warps' counts become the places of their positions
-  int k[SORT_WARPS], c = 0;
-  if (t < W)
-#pragma unroll
-    for (int i = 0; i < SORT_WARPS; ++i) k[i] = count[i * W + t];
-  if (t < W)
-#pragma unroll
-    for (int i = 0; i < SORT_WARPS; ++i) c += k[i];
-  int incl = c;  // scan over the tokens
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += u;
-  }
-  if (lane == 31) sh[w] = incl;
-  __syncthreads();
-  int first = base + incl - c;
-  for (int i = 0; i < w; ++i) first += sh[i];
-  if (t < W) {
-    e.start[(int64_t)me * W + t] = first;
-    int at = first;
-#pragma unroll
-    for (int i = 0; i < SORT_WARPS; ++i) {
-      count[i * W + t] = at;
-      at += k[i];
-    }
-    if (me == (int)gridDim.x - 1 && t == W - 1) e.start[(int64_t)gridDim.x * W] = first + c;
-  }
-  __syncthreads();
+  embed_places(e, count, me, base, sh);
   // 16 words at a time, a lane lists its word's hits, in order, as offsets from the
   // list's first word; a list that has grown long is placed, 32 hits at a time, a
   // lane each, the tokens of the next 32 under way.
@@ -267,20 +285,150 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
     for (int h = 0; h < have; h += 32) {
       const int next = fetch(h + 32 + lane), k = have - h < 32 ? have - h : 32;
       if (lane < k) {
-        const uint32_t some = k == 32 ? 0xffffffffu : (1u << k) - 1;
-        int32_t* c = &count[w * W + e.local(v)];
-        const uint32_t peers = __match_any_sync(some, v);
-        const int rank = __popc(peers & ((1u << lane) - 1)), to = *c;
-        __syncwarp(some);
-        if (rank == 0) *c = to + __popc(peers);
-        e.pos[to + rank] = (int32_t)(first + list[h + lane]);
-        e.tok[to + rank] = v;
+        const int to = embed_take(k == 32 ? 0xffffffffu : (1u << k) - 1, v, &count[w * W + e.local(v)]);
+        e.pos[to] = (int32_t)(first + list[h + lane]);
+        e.tok[to] = v;
       }
       __syncwarp();
       v = next;
     }
     have = 0;
     list0 = i + SORT_U;
+  }
+}
+
+// Of many ids, or of a vocabulary of more CTAs than SMs, reading all G times is too
+// much.  They are then split by owner first: each of B CTAs counts the owners in its
+// share of the positions; each, knowing all counts, moves its share to where it
+// belongs, order kept; and G CTAs sort what is theirs by token, which is all they
+// read.  (262144 ids of 32000 tokens: 28 us against 53.)
+struct EmbedSplit {
+  int64_t share;     // words of a CTA
+  int32_t* count;    // [B][G]
+  int32_t* first;    // [G + 1]: where an owner's positions start
+  int32_t* pos;      // [n], by owner
+  int32_t* tok;      // [n]
+};
+
+template <int KIND>
+__global__ void __launch_bounds__(SORT_NT) k_embed_count(const EmbedSort e, const EmbedSplit p) {
+  ::tp::pdl_enter();
+  __shared__ int32_t owners[1 << SPLIT_G];
+  const int G = 1 << e.g;
+  for (int i = threadIdx.x; i < G; i += SORT_NT) owners[i] = 0;
+  __syncthreads();
+  const int64_t from = blockIdx.x * p.share * 32, to = from + p.share * 32 < e.n ? from + p.share * 32 : e.n;
+#pragma unroll 4
+  for (int64_t i = from + threadIdx.x; i < to; i += SORT_NT) {
+    const int v = token_id(e.ids, KIND, i);
+    if (e.valid(v)) atomicAdd(&owners[e.owner(v)], 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G; i += SORT_NT) p.count[(int64_t)blockIdx.x * G + i] = owners[i];
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(SORT_NT) k_embed_split(const EmbedSort e, const EmbedSplit p) {
+  ::tp::pdl_enter();
+  extern __shared__ int32_t sort_sm[];  // [warps][G]: counts, then places
+  __shared__ int32_t all[1 << SPLIT_G], before[1 << SPLIT_G], sh[SORT_WARPS];
+  const int G = 1 << e.g, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  for (int i = t; i < SORT_WARPS * G; i += SORT_NT) sort_sm[i] = 0;
+  for (int i = t; i < G; i += SORT_NT) all[i] = before[i] = 0;
+  __syncthreads();
+  {  // of each owner: how many there are, and how many in the shares before this one
+    const int o = t & (G - 1);
+    int sum = 0, less = 0;
+#pragma unroll 8
+    for (int b = t >> e.g; b < (int)gridDim.x; b += SORT_NT >> e.g) {
+      const int c = p.count[(int64_t)b * G + o];
+      sum += c;
+      less += b < (int)blockIdx.x ? c : 0;
+    }
+    atomicAdd(&all[o], sum);
+    atomicAdd(&before[o], less);
+  }
+  const int64_t nwords = (e.n + 31) >> 5, from = blockIdx.x * p.share, to = from + p.share < nwords ? from + p.share : nwords;
+  const int64_t per = (p.share + SORT_WARPS - 1) / SORT_WARPS;
+  const int64_t w0 = from + per * w < to ? from + per * w : to, w1 = w0 + per < to ? w0 + per : to;
+  int32_t* mine = sort_sm + w * G;
+  auto token = [&](int64_t word) {
+    const int64_t i = word * 32 + lane;
+    const int v = i < e.n ? token_id(e.ids, KIND, i) : -1;
+    return e.valid(v) ? v : -1;
+  };
+#pragma unroll 4
+  for (int64_t i = w0; i < w1; ++i) {
+    const int v = token(i);
+    if (v >= 0) atomicAdd(&mine[e.owner(v)], 1);
+  }
+  __syncthreads();
+  int incl = t < G ? all[t] : 0;  // scan over the owners
+  const int own = incl;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) sh[w] = incl;
+  __syncthreads();
+  int first = incl - own;
+  for (int i = 0; i < w; ++i) first += sh[i];
+  if (t < G) {
+    if (blockIdx.x == 0) {
+      p.first[t] = first;
+      if (t == G - 1) p.first[G] = first + own;
+    }
+    int at = first + before[t];
+    for (int i = 0; i < SORT_WARPS; ++i) {
+      const int c = sort_sm[i * G + t];
+      sort_sm[i * G + t] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  int next = w0 < w1 ? token(w0) : -1;
+  for (int64_t i = w0; i < w1; ++i) {
+    const int v = next;
+    if (i + 1 < w1) next = token(i + 1);
+    const uint32_t some = __ballot_sync(0xffffffffu, v >= 0);
+    if (v >= 0) {
+      const int to = embed_take(some, e.owner(v), &mine[e.owner(v)]);
+      p.pos[to] = (int32_t)(i * 32 + lane);
+      p.tok[to] = v;
+    }
+    __syncwarp();
+  }
+}
+
+__global__ void __launch_bounds__(SORT_NT) k_embed_place(const EmbedSort e, const EmbedSplit p) {
+  ::tp::pdl_enter();
+  extern __shared__ int32_t sort_sm[];  // [warps][W]
+  __shared__ int32_t sh[SORT_WARPS];
+  const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  for (int i = t; i < SORT_WARPS * W; i += SORT_NT) sort_sm[i] = 0;
+  __syncthreads();
+  const int base = p.first[me], end = p.first[me + 1];
+  const int per = ((end - base + SORT_NT - 1) / SORT_NT) * 32;  // of a warp
+  const int64_t s0 = (int64_t)base + (int64_t)per * w;
+  const int64_t i0 = s0 < end ? s0 : end, i1 = i0 + per < end ? i0 + per : end;
+  int32_t* mine = sort_sm + w * W;
+#pragma unroll 4
+  for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[e.local(p.tok[i])], 1);
+  __syncthreads();
+  embed_places(e, sort_sm, me, base, sh);
+  int v = i0 + lane < i1 ? p.tok[i0 + lane] : -1, at = v >= 0 ? p.pos[i0 + lane] : 0;
+  for (int64_t i = i0; i < i1; i += 32) {
+    const bool more = i + 32 + lane < i1;
+    const int nv = more ? p.tok[i + 32 + lane] : -1, nat = more ? p.pos[i + 32 + lane] : 0;
+    const uint32_t some = __ballot_sync(0xffffffffu, v >= 0);
+    if (v >= 0) {
+      const int to = embed_take(some, v, &mine[e.local(v)]);
+      e.pos[to] = at;
+      e.tok[to] = v;
+    }
+    __syncwarp();
+    v = nv;
+    at = nat;
   }
 }
 
@@ -504,8 +652,9 @@ void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int
 }
 
 struct EmbedPlan {
-  int64_t per, start, pos, tok, cut, partial, ldp, bytes, tiles;
-  int g, T;
+  int64_t per, start, pos, tok, cut, count, first, spos, stok, partial, ldp, bytes, tiles, share;
+  int g, T, B;
+  bool split;
   EmbedPlan(int64_t n, int64_t V, int64_t D) {
     g = 7;  // 128 CTAs for 148 SMs
     while (((int64_t)SORT_TOKENS << g) < V) ++g;
@@ -518,7 +667,16 @@ struct EmbedPlan {
     pos = start + up(((per << g) + 1) * 4);
     tok = pos + up(n * 4 + 32);
     cut = tok + up(n * 4 + 32);
-    partial = cut + up(tiles * 8);
+    // the whole gradient at a width of 64: 32768 ids of 32000 tokens 24.8 us in one
+    // launch, 27.5 split first; 65536 ids 33.9 and 31.6
+    split = g <= SPLIT_G && n << g > (int64_t)1 << 22;
+    share = ((n + 31) / 32 + 147) / 148;
+    B = split ? (int)(((n + 31) / 32 + share - 1) / share) : 0;
+    count = cut + up(tiles * 8);
+    first = count + up((int64_t)B * 4 << g);
+    spos = first + (split ? up(4 + (4 << g)) : 0);
+    stok = spos + (split ? up(n * 4) : 0);
+    partial = stok + (split ? up(n * 4) : 0);
     bytes = partial + 2 * tiles * ldp * 4;
   }
 };
@@ -541,6 +699,16 @@ static void launch_sum(const EmbedSort& e, EmbedSum a, int64_t D) {
   const int jchunks = (int)((D + 127) / 128);
   TP_LAUNCH(k_embed_join<ACC>, grid_of((a.tiles + JOIN_TILES - 1) / JOIN_TILES, jchunks, what), dim3(32, JOIN_ROWS), 0,
             a, D, jchunks);
+}
+
+// Lets a kernel have that much dynamic shared memory; asked for once per kernel.
+template <class K>
+static void raise_smem(K* kernel, int bytes) {
+  static std::vector<void*> done;
+  for (void* k : done)
+    if (k == (void*)kernel) return;
+  TP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.push_back((void*)kernel);
 }
 
 void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
@@ -567,16 +735,29 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   e.start = (int32_t*)(base + p.start);
   e.pos = (int32_t*)(base + p.pos);
   e.tok = (int32_t*)(base + p.tok);
-  const int64_t words = (n + 31) / 32;
-  const size_t smem = (size_t)(SORT_WARPS * (p.per + SORT_LIST / 2) + (words <= SORT_WORDS ? words : 0)) * 4;
-  auto sort = kind == IDS_I32 ? k_embed_sort<IDS_I32> : k_embed_sort<IDS_F32>;
-  static bool raised[2] = {false, false};
-  if (!raised[kind]) {  // 128 KB of counts, 48 of listed hits, 32 of hits at most
-    TP_CUDA(cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (SORT_WARPS * (SORT_TOKENS + SORT_LIST / 2) + SORT_WORDS) * 4));
-    raised[kind] = true;
+  const bool i32 = kind == IDS_I32;
+  if (p.split) {
+    EmbedSplit s;
+    s.share = p.share;
+    s.count = (int32_t*)(base + p.count);
+    s.first = (int32_t*)(base + p.first);
+    s.pos = (int32_t*)(base + p.spos);
+    s.tok = (int32_t*)(base + p.stok);
+    raise_smem(k_embed_split<IDS_I32>, SORT_WARPS * 4 << SPLIT_G);
+    raise_smem(k_embed_split<IDS_F32>, SORT_WARPS * 4 << SPLIT_G);
+    raise_smem(k_embed_place, SORT_WARPS * 4 * SORT_TOKENS);
+    TP_LAUNCH(i32 ? k_embed_count<IDS_I32> : k_embed_count<IDS_F32>, p.B, SORT_NT, 0, e, s);
+    TP_LAUNCH(i32 ? k_embed_split<IDS_I32> : k_embed_split<IDS_F32>, p.B, SORT_NT, (size_t)SORT_WARPS * 4 << p.g, e, s);
+    TP_LAUNCH(k_embed_place, 1u << p.g, SORT_NT, (size_t)SORT_WARPS * 4 * p.per, e, s);
+  } else {
+    // at most 128 KB of counts, 48 of listed hits, 32 of hits
+    const int most = (SORT_WARPS * (SORT_TOKENS + SORT_LIST / 2) + SORT_WORDS) * 4;
+    const int64_t words = (n + 31) / 32;
+    const size_t smem = (size_t)(SORT_WARPS * (p.per + SORT_LIST / 2) + (words <= SORT_WORDS ? words : 0)) * 4;
+    raise_smem(k_embed_sort<IDS_I32>, most);
+    raise_smem(k_embed_sort<IDS_F32>, most);
+    TP_LAUNCH(i32 ? k_embed_sort<IDS_I32> : k_embed_sort<IDS_F32>, 1u << p.g, SORT_NT, smem, e);
   }
-  TP_LAUNCH(sort, 1u << p.g, SORT_NT, smem, e);
   EmbedSum a;
   a.dout = dout;
   a.ldo = ldo;
