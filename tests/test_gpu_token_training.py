@@ -171,6 +171,23 @@ def test_captured_step_replays_on_new_inputs(cuda_rt, n, V):
     assert rt.lib.tp_graph_destroy(g.value) == 0
 
 
+def test_plain_stream_order_gives_the_same_bits(cuda_rt):
+    """Without programmatic dependent launches (tp_set_pdl)."""
+    rt = cuda_rt
+    for n, V in ((140, 97), (24, 9001)):
+        E, W, *batch = make(V=V, n=n)
+        steps = []
+        for pdl in (1, 0):
+            assert rt.lib.tp_set_pdl(pdl) == 0
+            s = Step(rt, E, W, n)
+            s.feed(*batch)
+            s.run(1.5, 0.05)
+            rt.synchronize()
+            steps.append(s.outputs())
+        assert rt.lib.tp_set_pdl(1) == 0
+        assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(*steps))
+
+
 def test_two_steps_on_two_streams(cuda_rt):
     """The operators of two steps queued on the library's stream and on the
     auxiliary one at the same time, each with its own buffers."""

@@ -110,8 +110,8 @@ struct LpRow {
 // them): at least K logits are as large as the K-th largest of the lanes' maxima;
 // what is that large is collected and the K best of it are ranked by counting.
 // Where more is equal than the list holds, they are found one after the other.
-// 65536 x 258: 12.9 us without alternatives (10.5 at HBM's rate), 26 with three:
-// the compares that pick them out of registers are then what takes the time.
+// 65536 x 258: 12.9 us without alternatives (10.5 at HBM's rate), 19.8 with three:
+// what picks them out of the registers is then as long as the rest.
 template <int L, int N, bool TOP>
 __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict__ x, int64_t ld,
                                                         const void* __restrict__ ids, int kind, int64_t R, int V,
@@ -219,10 +219,10 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
 // cluster's CTAs take a part of one each; the parts' statistics meet in the
 // cluster's first CTA over distributed shared memory, so one launch serves one
 // row as well as many and no workspace is shared between calls.  (One row of
-// 32000 with 20 alternatives: 8.3 us in eight parts, 36 us by a warp.  2000 rows of
+// 32000 with 20 alternatives: 7.0 us in eight parts, 36 us by a warp.  2000 rows of
 // 50021 in two parts each: 95 us against 73, the exchange costs more than it
-// balances.)  1999 x 50021 with 5 alternatives: 70 us, 5.7 TB/s, of which the
-// alternatives are 10 and the last, uneven wave of rows most of the rest.
+// balances.)  1999 x 50021 with 5 alternatives: 70 us, 5.7 TB/s: the last, uneven
+// wave of rows is most of what is missing.
 //
 // The alternatives cost the walk next to nothing: each thread knows the maxima
 // of its four vectors (over all batches): four units.  With tau a value that at
