@@ -224,13 +224,14 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
 // balances.)  1999 x 50021 with 5 alternatives: 70 us, 5.7 TB/s: the last, uneven
 // wave of rows is most of what is missing.
 //
-// The alternatives cost the walk next to nothing: each thread knows the maxima
-// of its four vectors (over all batches): four units.  With tau a value that at
-// least K units reach, the K best logits all stand in units that reach it: these
-// are read again (from L2: one to four times K of the team's 4 NT), what reaches
-// tau is collected, and the K best of it are ranked by counting.  Where so many
-// logits are equal that the units or the collected logits do not fit their
-// lists, whole threads are told apart by the index of their maximum too, which
+// The alternatives cost the walk little: of the q-th vectors of all its batches (a
+// unit), each thread knows the largest maximum, where it stands and the largest of
+// the others.  With tau a value that at least K units reach, the K best logits all
+// stand in units that reach it.  Of such a unit one vector is read again, or all
+// where another of its vectors reaches tau too (the row has mostly left L2 by
+// then, so it matters how little that is); what reaches tau is collected, and the
+// K best of it are ranked by counting.  Where so many logits are equal that a list
+// overflows, whole threads are told apart by the index of their maximum too, which
 // leaves exactly K of them.
 
 // A part of a row as 16-byte vectors: vector j holds the logits 4 j - a ..
@@ -278,16 +279,16 @@ struct LpPart {
 template <int NT>
 struct LpShared {
   static constexpr int CAND = NT == 32 ? 256 : 512;  // collected logits
-  static constexpr int LIST = NT == 32 ? 128 : 256;  // units read again
+  static constexpr int LIST = NT == 32 ? 128 : 256;  // vectors, and units, read again
   LpStat warp[NT / 32];
   float kth[NT / 32];                  // per warp: a value that K / (NT / 32) of its threads' maxima reach
   unsigned long long top[LP_MAX_TOP];  // the part's alternatives
-  unsigned short chosen[LIST];         // the units read again: 4 thread + vector
-  float value[LIST], tau;              // and their maxima; the K-th largest of these
+  int vector[LIST];                    // vectors read again
+  unsigned short chosen[LIST];         // units read again whole: 4 thread + vector
   unsigned short owner[NT];            // ties: threads
   unsigned long long cand[CAND];
   unsigned long long k[NT / 32], least;
-  int units, cands;
+  int vectors, units, cands;
 };
 
 // Where the cluster's CTAs leave what their parts came to: in the first one.
@@ -447,62 +448,47 @@ __device__ __noinline__ void lp_select_ties(int t, const float* base, int a, int
   }
 }
 
-// The K best keys of the part into sh.top, by thread t of the team.  um: this
-// thread's unit maxima, mb: the batch its largest came from first, tau: a value
+// What a thread knows of the q-th vectors of its batches: the largest maximum, the
+// batch it came from first, and the largest of the others.
+struct LpUnit {
+  float m, next;
+  int batch;
+};
+
+// The K best keys of the part into sh.top, by thread t of the team.  tau: a value
 // that at least K units reach; the counters are 0.
 template <int NT>
-__device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int mb, float tau, int K,
-                          LpShared<NT>& sh) {
+__device__ void lp_select(int t, const LpPart<NT>& p, const LpUnit (&unit)[4], float tau, int K, LpShared<NT>& sh) {
   tau = fmaxf(tau, -FLT_MAX);  // masked logits are no alternatives
-  unsigned mine = 0u;
+  bool in = false;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) mine |= um[q] >= tau ? 1u << q : 0u;
-  const bool in = mine != 0u;
-  while (mine) {
-    const int q = __ffs(mine) - 1, i = atomicAdd(&sh.units, 1);
-    mine &= mine - 1;
-    if (i < LpShared<NT>::LIST) {
-      sh.chosen[i] = (unsigned short)(4 * t + q);
-      sh.value[i] = q == 0 ? um[0] : (q == 1 ? um[1] : (q == 2 ? um[2] : um[3]));
-    }
-  }
-  lp_sync<NT>();
-  int n = sh.units;
-  if (n <= LpShared<NT>::LIST && n > K && n * p.batches() > 2 * NT) {
-    // much to read: first the K-th largest of them, and only what reaches that
-    constexpr int PER = LpShared<NT>::LIST / NT;
-    unsigned short code[PER];
-    bool keep[PER];
-#pragma unroll
-    for (int c = 0; c < PER; ++c) {
-      const int u = t + c * NT;
-      keep[c] = false;
-      if (u < n) {
-        const float y = sh.value[u];
-        int above = 0, same = 0;
-        for (int j = 0; j < n; ++j) {
-          above += sh.value[j] > y;
-          same += sh.value[j] == y;
-        }
-        code[c] = sh.chosen[u];
-        keep[c] = above < K;
-        if (keep[c] && above + same >= K) sh.tau = y;
+  for (int q = 0; q < 4; ++q)
+    if (unit[q].m >= tau) {
+      in = true;
+      if (unit[q].next < tau) {
+        const int i = atomicAdd(&sh.vectors, 1);
+        if (i < LpShared<NT>::LIST) sh.vector[i] = 4 * NT * unit[q].batch + NT * q + t;
+      } else {
+        const int i = atomicAdd(&sh.units, 1);
+        if (i < LpShared<NT>::LIST) sh.chosen[i] = (unsigned short)(4 * t + q);
       }
     }
-    lp_sync<NT>();
-    if (t == 0) sh.units = 0;
-    lp_sync<NT>();
-    tau = sh.tau;
-#pragma unroll
-    for (int c = 0; c < PER; ++c)
-      if (keep[c]) sh.chosen[atomicAdd(&sh.units, 1)] = code[c];
-    lp_sync<NT>();
-    n = sh.units;
-  }
-  if (n <= LpShared<NT>::LIST) {
-    lp_reread<NT>(t, p, sh.chosen, n, [&](float x, uint32_t at) {
+  lp_sync<NT>();
+  const int vectors = sh.vectors, units = sh.units;
+  if (vectors <= LpShared<NT>::LIST && units <= LpShared<NT>::LIST) {
+    auto take = [&](float x, uint32_t at) {
       if (x >= tau) lp_add(sh, x, at);
-    });
+    };
+    for (int i = t; i < vectors; i += NT) {
+      const int j = sh.vector[i];
+      const float4 x = p.vec(j);
+      const uint32_t at = (uint32_t)(p.lo + 4 * j);
+      take(x.x, at);
+      take(x.y, at + 1);
+      take(x.z, at + 2);
+      take(x.w, at + 3);
+    }
+    if (units) lp_reread<NT>(t, p, sh.chosen, units, take);
     lp_sync<NT>();
     const int nc = sh.cands;
     if (nc <= LpShared<NT>::CAND) {
@@ -510,7 +496,13 @@ __device__ void lp_select(int t, const LpPart<NT>& p, const float (&um)[4], int 
       return;
     }
   }
-  lp_select_ties<NT>(t, p.base, p.a, p.end, p.lo, in ? fmaxf(fmaxf(um[0], um[1]), fmaxf(um[2], um[3])) : -INFINITY, mb, K, sh);
+  // the thread's largest, and where it came from first
+  float m = unit[0].m;
+  int mb = unit[0].batch;
+#pragma unroll
+  for (int q = 1; q < 4; ++q)
+    if (unit[q].m > m || (unit[q].m == m && unit[q].batch < mb)) m = unit[q].m, mb = unit[q].batch;
+  lp_select_ties<NT>(t, p.base, p.a, p.end, p.lo, in ? m : -INFINITY, mb, K, sh);
 }
 
 // p's place in the cluster's first CTA
@@ -567,8 +559,9 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
   const LpPart<NT> p(xr, lo, hi);
   const int batches = p.batches();
   LpStat s{-INFINITY, 0.0f, 0.0f};
-  float um[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  int mb = 0;
+  LpUnit unit[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) unit[q] = LpUnit{-INFINITY, -INFINITY, 0};
   float4 next[SPLIT ? 4 : 1];
   if constexpr (SPLIT) p.batch(0, t, next);
   for (int b = 0; b < batches; ++b) {
@@ -583,17 +576,19 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
     float m;
     if (TOP) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) um[q] = lp_max(um[q], lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
-      m = lp_max(lp_max(um[0], um[1]), lp_max(um[2], um[3]));
+      for (int q = 0; q < 4; ++q) {
+        const float y = lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w));
+        unit[q].next = fmaxf(unit[q].next, fminf(unit[q].m, y));
+        if (y > unit[q].m) unit[q].batch = b;
+        unit[q].m = lp_max(unit[q].m, y);
+      }
+      m = lp_max(lp_max(unit[0].m, unit[1].m), lp_max(unit[2].m, unit[3].m));
     } else {
       m = s.m;
 #pragma unroll
       for (int q = 0; q < 4; ++q) m = lp_max(m, lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
     }
-    if (m != s.m) {
-      s.move(m);
-      mb = b;
-    }
+    if (m != s.m) s.move(m);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       s.add(v[q].x);
@@ -622,7 +617,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
       tau = lp_sorted(own, lane);
       tau = __shfl_sync(0xffffffffu, tau, kq - 1);
     }
-    if (t == 0) sh.units = sh.cands = 0, sh.least = 0ull;
+    if (t == 0) sh.vectors = sh.units = sh.cands = 0, sh.least = 0ull;
   }
   if (WARPS > 1) {
     if (lane == 0) {
@@ -653,7 +648,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
   }
   if (TOP) {
     if (WARPS == 1) __syncwarp();
-    if (s.m < INFINITY) lp_select<NT>(t, p, um, mb, tau, K, sh);  // not with a NaN or +inf in the part
+    if (s.m < INFINITY) lp_select<NT>(t, p, unit, tau, K, sh);  // not with a NaN or +inf in the part
     lp_sync<NT>();
   }
   if (SPLIT) {
