@@ -192,12 +192,13 @@ def test_alternatives_wherever_they_stand(cuda_rt, V, K, shape):
     check(cuda_rt, np.stack([row, row[::-1], rng.standard_normal(V)]), [0, V - 1, V // 2], K)
 
 
-@pytest.mark.parametrize("R, V", [(2400, 1025), (2400, 2050), (2401, 4096), (2402, 8191), (900, 5000), (1000, 20001),
+@pytest.mark.parametrize("R, V", [(2400, 1025), (2400, 2050), (2401, 4096), (2402, 8191), (2368, 12289), (2400, 30001),
+                                  (900, 5000), (1000, 20001),
                                   (10000, 258), (5000, 500)])
 @pytest.mark.parametrize("K", [0, 3, 8, 20, 32])
 def test_alternatives_of_many_rows(cuda_rt, R, V, K):
     """The same patterns in batches, whose rows other teams of threads take:
-    warps for up to 8192 logits, CTAs of 128 threads, groups of lanes."""
+    warps, CTAs of 128 or 256 threads, groups of lanes."""
     rng = np.random.default_rng(R + V + K)
     rows = [bf16(pattern(s, V, max(K, 1), rng)) for s in SHAPES + ["normal"] * 5]
     mask = np.where(rng.random(V) < 0.97, -np.inf, rows[-1])

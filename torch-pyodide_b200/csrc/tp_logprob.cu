@@ -879,20 +879,25 @@ static void launch_cluster(void (*kernel)(KArgs...), unsigned grid, unsigned blo
   g_launches++;
 }
 
-// Threads of a row's team.  Times with 5 alternatives, in us, 512 MB of logits:
+// Threads of a row's team.  Times in us, 512 MB of logits, without / with 5 / with
+// 20 alternatives:
 //
-//            4096   8192  16384  50021 logits a row      1999 rows of 50021   64 rows of 4096
-//   warp       97     98    108    120                                  100               9.4
-//   128       153    112     99     98                                   70               5.4
-//   256       178    117     97     96                                   74               6.6
+//          4096         8192          12000         16384         24000          50021 logits a row
+//   warp   83/ 97/124   83/ 93/108    91/ 98/109    91/ 99/112    101/107/121    101/109/125
+//   128   101/153/166   87/112/120    89/108/111    88/102/105     86/ 98/102     93/101/103
+//   256   105/178/201   83/129/144    83/113/123    83/106/110     80/100/107     90/ 97/101
 //
-// A warp's row has no barrier, and its walk is long only if rows are few; 128
-// threads leave the last rows of a few hundred per SM wave less alone than 256.
-static int lp_threads(int64_t R, int64_t V) {
+// A warp's row has no barrier; more threads have fewer batches each, which is worth
+// more the fewer alternatives there are to pick.  1999 rows of 50021 with 5: 100, 70
+// and 74 us (the last rows of a wave are less alone with 128); 64 rows of 4096 with
+// 20: 9.4, 5.1 and 6.6.
+static int lp_threads(int64_t R, int64_t V, int K) {
   const int64_t sms = sm_count();
-  if (V <= 8192 && R >= 16 * sms) return 32;
-  if (V <= 4096) return 128;
-  return R >= 6 * sms && R < 16 * sms ? 128 : 256;
+  if (R >= 16 * sms) {
+    if (V <= (K ? 12288 : 8192)) return 32;
+    return K && V <= 24576 ? 128 : 256;
+  }
+  return V <= 4096 || R >= 6 * sms ? 128 : 256;
 }
 
 void launch_logprobs(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int64_t V, int K, float* logp,
@@ -916,7 +921,7 @@ void launch_logprobs(const float* x, int64_t ld, const void* ids, int kind, int6
 #undef TP_LP_GROUP
     return;
   }
-  const int nt = lp_threads(R, V);
+  const int nt = lp_threads(R, V, K);
   // more CTAs per row while the rows alone leave SMs empty and a part keeps half a batch
   int parts = 1;
   while (nt == 256 && parts < LP_MAX_PARTS && R * parts < 4 * (int64_t)sm_count() && V / (2 * parts) >= 2048) parts *= 2;
