@@ -132,7 +132,8 @@ def test_gradient_of_long_sums(cuda_rt):
 
 
 @pytest.mark.parametrize("n, V", [(600001, 3000), (40000, 1), (33000, 131072), (32769, 140000), (5000, 1000000),
-                                  (300001, 2 ** 20 + 5), (20000, 2 ** 20 + 5)])
+                                  (300001, 2 ** 20 + 5), (20000, 2 ** 20 + 5), (70001, 3 * 2 ** 20 + 17),
+                                  (600001, 2 ** 22), (1, 2 ** 22 - 1)])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_gradient_of_many_tokens(cuda_rt, n, V, accumulate):
     """Ids that are split by owner before they are sorted, and more positions than
@@ -149,6 +150,15 @@ def test_gradient_vocabularies(cuda_rt, V):
     rng = np.random.default_rng(V)
     for n in (3, 3000):
         check_grad(cuda_rt, rng.standard_normal((n, 8)), rng.integers(0, V, n), V)
+
+
+@pytest.mark.parametrize("n", [0, 5, 3000])
+def test_gradient_largest_vocabulary(cuda_rt, n):
+    """Owners of 16384 tokens, which sort them in parts; the last id of each part, and of the table."""
+    V = 2 ** 24
+    ids = np.random.default_rng(n).integers(0, V, n)
+    ids[:4] = [V - 1, 0, 2 ** 20 - 1, 2 ** 20][:n]
+    check_grad(cuda_rt, np.random.default_rng(1).standard_normal((n, 1)), ids, V)
 
 
 def test_gradient_untouched_rows_keep_their_bits(cuda_rt):

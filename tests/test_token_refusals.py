@@ -34,7 +34,9 @@ LOGPROBS = dict(logits=P, ld=100, ids=P, kind=1, rows=4, vocab=100, topk=3, logp
     (dict(vocab=2 ** 24 + 1, ld=2 ** 25), "vocabulary"), (dict(ld=99), "row stride"), (dict(topk=-1), "topk"),
     (dict(topk=33), "topk"), (dict(vocab=2, topk=3), "topk"), (dict(kind=2), "ids_kind"), (dict(kind=-1), "ids_kind"),
     (dict(logits=None), "logits"), (dict(ids=None), "token ids"), (dict(top_ids=None), "alternatives"),
-    (dict(top_logp=None), "alternatives"), (dict(logits=P + 2), "aligned")])
+    (dict(top_logp=None), "alternatives"), (dict(logits=P + 2), "aligned"), (dict(ids=P + 1), "aligned"),
+    (dict(logp=P + 2), "aligned"), (dict(entropy=P + 2), "aligned"), (dict(stats=P + 2), "aligned"),
+    (dict(top_ids=P + 2), "aligned"), (dict(top_logp=P + 3), "aligned")])
 def test_logprobs(lib, change, word):
     refused(lib, lib.tpk_token_logprobs(*{**LOGPROBS, **change}.values()), word)
 
@@ -47,7 +49,8 @@ BACKWARD = dict(logits=P, ld=100, ids=P, kind=1, stats=P, entropy=P, dlogp=P, de
     (dict(rows=-1), "rows"), (dict(vocab=0), "vocabulary"), (dict(ld=99), "row stride"), (dict(ldd=99), "row stride"),
     (dict(kind=3), "ids_kind"), (dict(logits=None), "NULL"), (dict(stats=None), "NULL"), (dict(dlogits=None), "NULL"),
     (dict(ids=None), "token ids"), (dict(entropy=None), "entropy"), (dict(dlogits=P, ldd=101), "in place"),
-    (dict(dlogits=P + 1), "aligned")])
+    (dict(dlogits=P + 1), "aligned"), (dict(ids=P + 2), "aligned"), (dict(stats=P + 2), "aligned"),
+    (dict(entropy=P + 2), "aligned"), (dict(dlogp=P + 1), "aligned"), (dict(dentropy=P + 2), "aligned")])
 def test_logprobs_backward(lib, change, word):
     refused(lib, lib.tpk_token_logprobs_backward(*{**BACKWARD, **change}.values()), word)
 

@@ -138,7 +138,7 @@ constexpr int SORT_WARPS = SORT_NT / 32;
 constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a thread each in the scan)
 constexpr int SORT_WORDS = 8192;          // positions / 32 whose hits are kept in shared memory
 constexpr int SORT_LIST = 768;            // hits that a warp lists before it places them
-constexpr int SPLIT_G = 10;               // log2 of the owners that ids can be split by first
+constexpr int MOST_G = 10;                // log2 of the most CTAs
 constexpr int SORT_U = 16;                // ids of a thread in flight, and words listed at once
 
 struct EmbedSort {
@@ -157,10 +157,12 @@ struct EmbedSort {
   __device__ __forceinline__ int total() const { return start[(int64_t)per << g]; }
 };
 
-// The counts [warps][W] of CTA `me`'s tokens become the places of each warp's
-// positions, those of its first token starting at `base`; start[] is written.
-__device__ __forceinline__ void embed_places(const EmbedSort& e, int32_t* count, int me, int base, int32_t* sh) {
-  const int W = e.per, t = threadIdx.x, lane = t & 31, w = t >> 5;
+// The counts [warps][W] of CTA `me`'s tokens l0 .. l0 + W - 1 become the places of
+// each warp's positions, those of the first token starting at `base`; start[] is
+// written.  Returns where the last token's end.
+__device__ __forceinline__ int embed_places(const EmbedSort& e, int32_t* count, int me, int l0, int W, int base,
+                                            int32_t* sh) {
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   int k[SORT_WARPS], c = 0;  // one thread per token
   if (t < W)
 #pragma unroll
@@ -175,19 +177,21 @@ __device__ __forceinline__ void embed_places(const EmbedSort& e, int32_t* count,
   }
   if (lane == 31) sh[w] = incl;
   __syncthreads();
-  int first = base + incl - c;
+  int first = base + incl - c, end = base;
   for (int i = 0; i < w; ++i) first += sh[i];
+  for (int i = 0; i < SORT_WARPS; ++i) end += sh[i];
   if (t < W) {
-    e.start[(int64_t)me * W + t] = first;
+    e.start[(int64_t)me * e.per + l0 + t] = first;
     int at = first;
 #pragma unroll
     for (int i = 0; i < SORT_WARPS; ++i) {
       count[i * W + t] = at;
       at += k[i];
     }
-    if (me == (1 << e.g) - 1 && t == W - 1) e.start[(int64_t)W << e.g] = first + c;
+    if (me == (1 << e.g) - 1 && l0 + t == e.per - 1) e.start[(int64_t)e.per << e.g] = first + c;
   }
   __syncthreads();
+  return end;
 }
 
 // Where this lane's key stands: its place among the lanes of `some` (the ones that
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   int base = 0;
   for (int i = 0; i < SORT_WARPS; ++i) base += sh[i];
   __syncthreads();
-  embed_places(e, count, me, base, sh);
+  embed_places(e, count, me, 0, W, base, sh);
   // 16 words at a time, a lane lists its word's hits, in order, as offsets from the
   // list's first word; a list that has grown long is placed, 32 hits at a time, a
   // lane each, the tokens of the next 32 under way.
@@ -301,7 +305,10 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
 // much.  They are then split by owner first: each of B CTAs counts the owners in its
 // share of the positions; each, knowing all counts, moves its share to where it
 // belongs, order kept; and G CTAs sort what is theirs by token, which is all they
-// read.  (262144 ids of 32000 tokens: 28 us against 53.)
+// read.  (262144 ids of 32000 tokens: 28 us against 53.)  Owners of more tokens than
+// a CTA sorts at once (a vocabulary above 2^20) go through theirs again for each
+// SORT_TOKENS of them (262144 ids of 2 million tokens, 64 wide, added: 151 us; with
+// 2048 owners that each read all ids 552; 16384 ids: 91 and 98).
 struct EmbedSplit {
   int64_t share;     // words of a CTA
   int32_t* count;    // [B][G]
@@ -313,7 +320,7 @@ struct EmbedSplit {
 template <int KIND>
 __global__ void __launch_bounds__(SORT_NT) k_embed_count(const EmbedSort e, const EmbedSplit p) {
   ::tp::pdl_enter();
-  __shared__ int32_t owners[1 << SPLIT_G];
+  __shared__ int32_t owners[1 << MOST_G];
   const int G = 1 << e.g;
   for (int i = threadIdx.x; i < G; i += SORT_NT) owners[i] = 0;
   __syncthreads();
@@ -331,7 +338,7 @@ template <int KIND>
 __global__ void __launch_bounds__(SORT_NT) k_embed_split(const EmbedSort e, const EmbedSplit p) {
   ::tp::pdl_enter();
   extern __shared__ int32_t sort_sm[];  // [warps][G]: counts, then places
-  __shared__ int32_t all[1 << SPLIT_G], before[1 << SPLIT_G], sh[SORT_WARPS];
+  __shared__ int32_t all[1 << MOST_G], before[1 << MOST_G], sh[SORT_WARPS];
   const int G = 1 << e.g, t = threadIdx.x, lane = t & 31, w = t >> 5;
   for (int i = t; i < SORT_WARPS * G; i += SORT_NT) sort_sm[i] = 0;
   for (int i = t; i < G; i += SORT_NT) all[i] = before[i] = 0;
@@ -402,33 +409,43 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_split(const EmbedSort e, cons
 
 __global__ void __launch_bounds__(SORT_NT) k_embed_place(const EmbedSort e, const EmbedSplit p) {
   ::tp::pdl_enter();
-  extern __shared__ int32_t sort_sm[];  // [warps][W]
+  extern __shared__ int32_t sort_sm[];  // [warps][W], W tokens at once
   __shared__ int32_t sh[SORT_WARPS];
-  const int W = e.per, me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
-  for (int i = t; i < SORT_WARPS * W; i += SORT_NT) sort_sm[i] = 0;
-  __syncthreads();
-  const int base = p.first[me], end = p.first[me + 1];
-  const int per = ((end - base + SORT_NT - 1) / SORT_NT) * 32;  // of a warp
-  const int64_t s0 = (int64_t)base + (int64_t)per * w;
+  const int me = blockIdx.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  const int begin = p.first[me], end = p.first[me + 1];
+  const int per = ((end - begin + SORT_NT - 1) / SORT_NT) * 32;  // of a warp
+  const int64_t s0 = (int64_t)begin + (int64_t)per * w;
   const int64_t i0 = s0 < end ? s0 : end, i1 = i0 + per < end ? i0 + per : end;
-  int32_t* mine = sort_sm + w * W;
+  int base = begin;
+  for (int l0 = 0; l0 < e.per; l0 += SORT_TOKENS) {
+    const int W = e.per - l0 < SORT_TOKENS ? e.per - l0 : SORT_TOKENS;
+    for (int i = t; i < SORT_WARPS * W; i += SORT_NT) sort_sm[i] = 0;
+    __syncthreads();
+    int32_t* mine = sort_sm + w * W;
+    auto local = [&](int v) { return e.local(v) - l0; };
 #pragma unroll 4
-  for (int64_t i = i0 + lane; i < i1; i += 32) atomicAdd(&mine[e.local(p.tok[i])], 1);
-  __syncthreads();
-  embed_places(e, sort_sm, me, base, sh);
-  int v = i0 + lane < i1 ? p.tok[i0 + lane] : -1, at = v >= 0 ? p.pos[i0 + lane] : 0;
-  for (int64_t i = i0; i < i1; i += 32) {
-    const bool more = i + 32 + lane < i1;
-    const int nv = more ? p.tok[i + 32 + lane] : -1, nat = more ? p.pos[i + 32 + lane] : 0;
-    const uint32_t some = __ballot_sync(0xffffffffu, v >= 0);
-    if (v >= 0) {
-      const int to = embed_take(some, v, &mine[e.local(v)]);
-      e.pos[to] = at;
-      e.tok[to] = v;
+    for (int64_t i = i0 + lane; i < i1; i += 32) {
+      const int l = local(p.tok[i]);
+      if ((uint32_t)l < (uint32_t)W) atomicAdd(&mine[l], 1);
     }
-    __syncwarp();
-    v = nv;
-    at = nat;
+    __syncthreads();
+    base = embed_places(e, sort_sm, me, l0, W, base, sh);
+    int v = i0 + lane < i1 ? p.tok[i0 + lane] : -1, at = v >= 0 ? p.pos[i0 + lane] : 0;
+    for (int64_t i = i0; i < i1; i += 32) {
+      const bool more = i + 32 + lane < i1;
+      const int nv = more ? p.tok[i + 32 + lane] : -1, nat = more ? p.pos[i + 32 + lane] : 0;
+      const bool take = v >= 0 && (uint32_t)local(v) < (uint32_t)W;
+      const uint32_t some = __ballot_sync(0xffffffffu, take);
+      if (take) {
+        const int to = embed_take(some, v, &mine[local(v)]);
+        e.pos[to] = at;
+        e.tok[to] = v;
+      }
+      __syncwarp();
+      v = nv;
+      at = nat;
+    }
+    __syncthreads();
   }
 }
 
@@ -657,7 +674,7 @@ struct EmbedPlan {
   bool split;
   EmbedPlan(int64_t n, int64_t V, int64_t D) {
     g = 7;  // 128 CTAs for 148 SMs
-    while (((int64_t)SORT_TOKENS << g) < V) ++g;
+    while (g < MOST_G && ((int64_t)SORT_TOKENS << g) < V) ++g;
     per = (V + (1 << g) - 1) >> g;
     T = n / 64 * D >= 148 * 8 * 512 ? 64 : 16;  // 512 values of a row to a CTA, 8 CTAs to an SM
     tiles = (n + T - 1) / T;
@@ -669,9 +686,10 @@ struct EmbedPlan {
     cut = tok + up(n * 4 + 32);
     // the whole gradient at a width of 64: 32768 ids of 32000 tokens 24.8 us in one
     // launch, 27.5 split first; 65536 ids 33.9 and 31.6
-    split = g <= SPLIT_G && n << g > (int64_t)1 << 22;
-    share = ((n + 31) / 32 + 147) / 148;
-    B = split ? (int)(((n + 31) / 32 + share - 1) / share) : 0;
+    split = per > SORT_TOKENS || n << g > (int64_t)1 << 22;
+    const int64_t words = n > 0 ? (n + 31) / 32 : 1;
+    share = (words + 147) / 148;
+    B = split ? (int)((words + share - 1) / share) : 0;
     count = cut + up(tiles * 8);
     first = count + up((int64_t)B * 4 << g);
     spos = first + (split ? up(4 + (4 << g)) : 0);
@@ -743,12 +761,13 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
     s.first = (int32_t*)(base + p.first);
     s.pos = (int32_t*)(base + p.spos);
     s.tok = (int32_t*)(base + p.stok);
-    raise_smem(k_embed_split<IDS_I32>, SORT_WARPS * 4 << SPLIT_G);
-    raise_smem(k_embed_split<IDS_F32>, SORT_WARPS * 4 << SPLIT_G);
+    raise_smem(k_embed_split<IDS_I32>, SORT_WARPS * 4 << MOST_G);
+    raise_smem(k_embed_split<IDS_F32>, SORT_WARPS * 4 << MOST_G);
     raise_smem(k_embed_place, SORT_WARPS * 4 * SORT_TOKENS);
     TP_LAUNCH(i32 ? k_embed_count<IDS_I32> : k_embed_count<IDS_F32>, p.B, SORT_NT, 0, e, s);
     TP_LAUNCH(i32 ? k_embed_split<IDS_I32> : k_embed_split<IDS_F32>, p.B, SORT_NT, (size_t)SORT_WARPS * 4 << p.g, e, s);
-    TP_LAUNCH(k_embed_place, 1u << p.g, SORT_NT, (size_t)SORT_WARPS * 4 * p.per, e, s);
+    const int64_t W = p.per < SORT_TOKENS ? p.per : SORT_TOKENS;
+    TP_LAUNCH(k_embed_place, 1u << p.g, SORT_NT, (size_t)SORT_WARPS * 4 * W, e, s);
   } else {
     // at most 128 KB of counts, 48 of listed hits, 32 of hits
     const int most = (SORT_WARPS * (SORT_TOKENS + SORT_LIST / 2) + SORT_WORDS) * 4;
@@ -797,8 +816,7 @@ TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, 
     check_ids_kind(ids_kind, what);
     if (n == 0 || dim == 0) return;
     TP_REQUIRE(table && ids && out, "%s: table, ids and out must not be NULL", what);
-    TP_REQUIRE((((uintptr_t)table | (uintptr_t)ids | (uintptr_t)out) & 3) == 0, "%s: a buffer is not 4-byte aligned",
-               what);
+    check_aligned({table, ids, out}, what);
     TP_REQUIRE(out != table && (const void*)out != ids, "%s: out is an input", what);
     launch_embed(table, ld, ids, ids_kind, n, vocab, dim, scale, out, ldo);
   });
@@ -824,8 +842,7 @@ TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const vo
     TP_REQUIRE(accumulate == 0 || accumulate == 1, "%s: accumulate must be 0 or 1, got %d", what, accumulate);
     if (dim == 0) return;
     TP_REQUIRE(dtable && (n == 0 || (dout && ids)), "%s: dout, ids and dtable must not be NULL", what);
-    TP_REQUIRE((((uintptr_t)dout | (uintptr_t)ids | (uintptr_t)dtable) & 3) == 0,
-               "%s: a buffer is not 4-byte aligned", what);
+    check_aligned({dout, ids, dtable}, what);
     TP_REQUIRE(dtable != dout && (const void*)dtable != ids, "%s: dtable is an input", what);
     const int64_t need = embed_bwd_ws(n, vocab, dim);
     TP_REQUIRE(ws_bytes >= need && (need == 0 || ws), "%s: a workspace of %lld bytes, %lld are needed", what,

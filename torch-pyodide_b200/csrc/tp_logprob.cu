@@ -991,7 +991,7 @@ TP_API int tpk_token_logprobs(const float* logits, int64_t ld, const void* ids, 
     TP_REQUIRE(logits, "%s: logits is NULL", what);
     TP_REQUIRE(!logp || ids, "%s: log-probabilities need token ids", what);
     TP_REQUIRE(topk == 0 || (top_ids && top_logp), "%s: topk > 0 needs both outputs of the alternatives", what);
-    TP_REQUIRE(((uintptr_t)logits & 3) == 0, "%s: logits are not 4-byte aligned", what);
+    check_aligned({logits, ids, logp, entropy, stats, top_ids, top_logp}, what);
     launch_logprobs(logits, ld, ids, ids_kind, rows, vocab, topk, logp, entropy, stats, top_ids, top_logp);
   });
 }
@@ -1009,7 +1009,7 @@ TP_API int tpk_token_logprobs_backward(const float* logits, int64_t ld, const vo
     TP_REQUIRE(logits && stats && dlogits, "%s: logits, stats and dlogits must not be NULL", what);
     TP_REQUIRE(!dlogp || ids, "%s: a gradient of log-probabilities needs token ids", what);
     TP_REQUIRE(!dentropy || entropy, "%s: a gradient of the entropy needs the entropy", what);
-    TP_REQUIRE((((uintptr_t)logits | (uintptr_t)dlogits) & 3) == 0, "%s: a buffer is not 4-byte aligned", what);
+    check_aligned({logits, ids, stats, entropy, dlogp, dentropy, dlogits}, what);
     TP_REQUIRE(dlogits != logits || ldd == ld, "%s: in place needs the same row stride", what);
     launch_logprobs_bwd(logits, ld, ids, ids_kind, stats, entropy, dlogp, dentropy, rows, vocab, dlogits, ldd);
   });

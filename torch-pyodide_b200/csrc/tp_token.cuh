@@ -40,6 +40,11 @@ inline void check_vocab(int64_t V, const char* what) {
   TP_REQUIRE(V >= 1 && V <= TOKEN_MAX_VOCAB, "%s: a vocabulary of %lld is outside [1, 2^24]", what, (long long)V);
 }
 
+// Every value of a caller's buffers is 4 bytes; nothing more is asked of them.
+inline void check_aligned(std::initializer_list<const void*> buffers, const char* what) {
+  for (const void* p : buffers) TP_REQUIRE(((uintptr_t)p & 3) == 0, "%s: a buffer is not 4-byte aligned", what);
+}
+
 // Output tensors of one call: freed again if the call throws before they are
 // registered.
 class Outputs {
