@@ -46,36 +46,34 @@ static int block_cols(int64_t cols) {
 }
 
 // ---- lookup ---------------------------------------------------------------------------
-// A CTA per 512 columns of a row (or several narrow rows): the id, then the row,
-// are fetched one after the other, so it takes many CTAs to keep HBM busy.
-// 32768 x 2048: 59.5 us, 6.0 TB/s read and written.
-constexpr int EMB_U = 4;  // columns per thread, loaded before the first is stored
+// A row to up to 128 threads of a CTA, several columns each, all loaded before the
+// first is stored; the rest of its 256 threads take other rows, since SMs start
+// CTAs only so fast (85921 x 535 by CTAs of one row 178 us, of 4 rows 54).  Offsets
+// are 32-bit and step by the CTA's width: rows that are no multiple of 16 bytes
+// are bound by instructions.  32768 x 2048: 59.6 us, 6.0 TB/s read and written.
+constexpr int LOOK_NT = 256, LOOK_TX = 128;
 
-template <int VEC>
-__global__ void __launch_bounds__(EMB_NT) k_embed(const float* __restrict__ table, int64_t ld,
-                                                  const void* __restrict__ ids, int kind, int64_t n, int64_t V,
-                                                  int64_t cols, int chunks, float scale, float* __restrict__ out,
+template <int VEC, int U>  // U: columns per thread, loaded before the first is stored
+__global__ void __launch_bounds__(LOOK_NT) k_embed(const float* __restrict__ table, int64_t ld,
+                                                  const void* __restrict__ ids, int kind, int64_t n, int V,
+                                                  uint32_t cols, int chunks, float scale, float* __restrict__ out,
                                                   int64_t ldo) {
   ::tp::pdl_enter();
-  const int64_t group = blockIdx.x / chunks;
-  const int64_t i = group * blockDim.y + threadIdx.y;
-  const int64_t c0 = (int64_t)(blockIdx.x - group * chunks) * EMB_U * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  const int64_t v = token_id(ids, kind, i);
+  const uint32_t group = chunks == 1 ? blockIdx.x : blockIdx.x / (uint32_t)chunks, tx = blockDim.x;
+  const int64_t i = (int64_t)group * blockDim.y + threadIdx.y;
+  const uint32_t c0 = (blockIdx.x - group * chunks) * U * tx + threadIdx.x;
+  if (i >= n || c0 >= cols) return;
+  const uint32_t left = cols - c0;
+  const int v = token_id(ids, kind, i);
   const bool in = v >= 0 && v < V;
-  const float* src = table + v * ld;
-  float* dst = out + i * ldo;
-  Col<VEC> x[EMB_U];
+  const float* src = table + v * ld + (int64_t)VEC * c0;
+  float* dst = out + i * ldo + (int64_t)VEC * c0;
+  Col<VEC> x[U];
 #pragma unroll
-  for (int u = 0; u < EMB_U; ++u) {
-    const int64_t c = c0 + u * (int)blockDim.x;
-    if (in && c < cols) x[u] = Col<VEC>::load(src, c);
-  }
+  for (int u = 0; u < U; ++u) x[u] = in && u * tx < left ? Col<VEC>::load(src, u * tx) : Col<VEC>::zero().times(NAN);
 #pragma unroll
-  for (int u = 0; u < EMB_U; ++u) {
-    const int64_t c = c0 + u * (int)blockDim.x;
-    if (c < cols) (in ? x[u].times(scale) : Col<VEC>::zero().times(NAN)).store(dst, c);
-  }
+  for (int u = 0; u < U; ++u)
+    if (u * tx < left) x[u].times(scale).store(dst, u * tx);
 }
 
 // ---- gradient of a few tokens, added to an existing one -----------------------------------
@@ -661,11 +659,21 @@ void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int
   if (n == 0 || D == 0) return;
   const bool vec = D % 4 == 0 && aligned_rows(table, ld) && aligned_rows(out, ldo);
   const int64_t cols = vec ? D / 4 : D;
-  const int tx = block_cols((cols + EMB_U - 1) / EMB_U), ty = EMB_NT / tx;
-  const int chunks = (int)((cols + EMB_U * tx - 1) / (EMB_U * tx));
+  // columns of a thread; 20000 x 777 by 16 17.5 us, by 8 21.2; 200000 x 33 14.3 and 10.7
+  const int U = vec ? 4 : (cols > 512 ? 16 : 8);
+  const int64_t need = (cols + U - 1) / U;  // threads
+  const int chunks = (int)((need + LOOK_TX - 1) / LOOK_TX);
+  int tx = block_cols(need);
+  if (tx > 32) tx = (int)(((need + chunks - 1) / chunks + 31) / 32 * 32);
+  const int ty = LOOK_NT / tx;
   const unsigned grid = grid_of((n + ty - 1) / ty, chunks, "token_embedding");
-  if (vec) TP_LAUNCH(k_embed<4>, grid, dim3(tx, ty), 0, table, ld, ids, kind, n, V, cols, chunks, scale, out, ldo);
-  else TP_LAUNCH(k_embed<1>, grid, dim3(tx, ty), 0, table, ld, ids, kind, n, V, cols, chunks, scale, out, ldo);
+#define TP_EMBED(VEC, U)                                                                                         \
+  TP_LAUNCH((k_embed<VEC, U>), grid, dim3(tx, ty), 0, table, ld, ids, kind, n, (int)V, (uint32_t)cols, chunks, scale, \
+            out, ldo)
+  if (vec) TP_EMBED(4, 4);
+  else if (U == 16) TP_EMBED(1, 16);
+  else TP_EMBED(1, 8);
+#undef TP_EMBED
 }
 
 struct EmbedPlan {
