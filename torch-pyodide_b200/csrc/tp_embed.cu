@@ -15,7 +15,8 @@
 
 namespace tp {
 
-// A column of a row: 4 values where rows start on 16-byte boundaries, else 1.
+// A column of a row: 4 values where rows start on 16-byte boundaries, 2 where they
+// do on 8-byte ones, else 1.
 template <int VEC>
 struct Col;
 template <>
@@ -26,6 +27,15 @@ struct Col<4> {
   __device__ __forceinline__ Col times(float s) const { return {make_float4(v.x * s, v.y * s, v.z * s, v.w * s)}; }
   __device__ static Col load(const float* p, int64_t c) { return {*(reinterpret_cast<const float4*>(p) + c)}; }
   __device__ void store(float* p, int64_t c) const { *(reinterpret_cast<float4*>(p) + c) = v; }
+};
+template <>
+struct Col<2> {
+  float2 v;
+  __device__ static Col zero() { return {make_float2(0.0f, 0.0f)}; }
+  __device__ __forceinline__ void add(const Col& o) { v.x += o.v.x, v.y += o.v.y; }
+  __device__ __forceinline__ Col times(float s) const { return {make_float2(v.x * s, v.y * s)}; }
+  __device__ static Col load(const float* p, int64_t c) { return {*(reinterpret_cast<const float2*>(p) + c)}; }
+  __device__ void store(float* p, int64_t c) const { *(reinterpret_cast<float2*>(p) + c) = v; }
 };
 template <>
 struct Col<1> {
@@ -76,20 +86,66 @@ __global__ void __launch_bounds__(LOOK_NT) k_embed(const float* __restrict__ tab
     if (u * tx < left) x[u].times(scale).store(dst, u * tx);
 }
 
-// ---- gradient of a few tokens, added to an existing one -----------------------------------
+// Clears a row of D values by n threads, this one the t-th: 16-byte stores between
+// its ends.
+__device__ __forceinline__ void clear_row(float* row, int64_t D, int t, int n) {
+  int64_t head = (4 - (((uintptr_t)row >> 2) & 3)) & 3;
+  if (head > D) head = D;
+  const int64_t body = (D - head) >> 2;
+  if (t < head) row[t] = 0.0f;
+  float4* mid = reinterpret_cast<float4*>(row + head);
+#pragma unroll 4
+  for (int64_t q = t; q < body; q += n) mid[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (t < D - head - 4 * body) row[head + 4 * body + t] = 0.0f;
+}
+
+// ---- gradient of a few tokens ---------------------------------------------------------
 // One CTA per (position, 256 columns), which compares its token with all ids at
 // once: the first position of a token sums all of them, in order.  Reads the ids
-// n times over, and a frequent token's rows one after the other: 256 x 1024 takes
-// 5.7 us against 14.1 sorted, 1024 x 4096 23.6 against 22.5.
+// n times over, and a frequent token's rows by one thread per column: 256 x 1024
+// takes 5.2 us against 14.1 sorted, 1024 x 4096 23.6 against 22.5, 512 x 1024 all of
+// one token 39.  Where rows are written, not added to, more CTAs clear `clear` rows
+// each that no id names (2 x 2846 into 3946 rows: 7.8 us, 35 sorted).
 constexpr int EMB_FEW = 512;
+constexpr int FEW_U = 16;  // rows in flight (500 x 4096 of 10 tokens, added: 11.4 us, 14.4 with 8)
+constexpr int FEW_CLEAR = 1024;       // rows that a CTA looks at, at most
+constexpr int FEW_CLEAR_VALUES = 8192;  // values that it clears, if rows are shorter
 
-template <int VEC>
+template <int VEC, bool ACC>
 __global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dout, int64_t ldo,
                                                    const void* __restrict__ ids, int kind, int n, int64_t V,
                                                    int64_t cols, int chunks, float scale, int64_t pad,
-                                                   float* __restrict__ dtable, int64_t ld) {
+                                                   float* __restrict__ dtable, int64_t ld, int clear) {
   ::tp::pdl_enter();
+  if (!ACC && blockIdx.x >= (unsigned)n * chunks) {
+    __shared__ bool present[FEW_CLEAR];
+    const int t = threadIdx.x;
+    const int64_t v0 = (int64_t)(blockIdx.x - (unsigned)n * chunks) * clear, D = cols * VEC;
+    const int rows = (int)(V - v0 < clear ? V - v0 : clear);
+    for (int r = t; r < rows; r += 256) present[r] = false;
+    __syncthreads();
+    for (int i = t; i < n; i += 256) {
+      const int v = token_id(ids, kind, i);
+      if (v >= v0 && v < v0 + rows && v != pad) present[v - v0] = true;
+    }
+    __syncthreads();
+    float* first = dtable + v0 * ld;
+    if (D < 32) {
+      for (int e = t; e < rows * (int)D; e += 256) {
+        const int r = e / (int)D;
+        if (!present[r]) first[r * ld + e - r * (int)D] = 0.0f;
+      }
+    } else if (clear >= 8) {  // a warp per row
+      for (int r = t >> 5; r < rows; r += 8)
+        if (!present[r]) clear_row(first + r * ld, D, t & 31, 32);
+    } else {
+      for (int r = 0; r < rows; ++r)
+        if (!present[r]) clear_row(first + r * ld, D, t, 256);
+    }
+    return;
+  }
   __shared__ uint32_t hits[EMB_FEW / 32];
+  __shared__ uint16_t list[EMB_FEW];
   const int t = threadIdx.x, lane = t & 31;
   const int i = blockIdx.x / chunks;
   const int64_t c = (int64_t)(blockIdx.x - i * chunks) * 256 + t;
@@ -106,19 +162,37 @@ __global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dou
     if (lane == 0) hits[r * 8 + (t >> 5)] = b;
   }
   if (__syncthreads_or(earlier)) return;
-  if (c >= cols) return;
-  const Col<VEC> old = Col<VEC>::load(dtable + (int64_t)v * ld, c);
-  Col<VEC> acc = Col<VEC>::zero();
-  for (int w0 = i >> 8 << 3; 32 * w0 < n; w0 += 8) {  // chains of at most 256 additions, then of n / 256
-    Col<VEC> part = Col<VEC>::zero();
+  int many = 0;  // the token's positions, in order
 #pragma unroll
-    for (int w = w0; w < w0 + 8; ++w)
-      for (uint32_t q = hits[w]; q; q &= q - 1)
-        part.add(Col<VEC>::load(dout + (int64_t)(32 * w + __ffs(q) - 1) * ldo, c));
-    acc.add(part);
+  for (int r = 0; r < EMB_FEW / 256; ++r) {
+    int at = many;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const int k = __popc(hits[r * 8 + w]);
+      at += w < t >> 5 ? k : 0;
+      many += k;
+    }
+    if (u[r] == v) list[at + __popc(hits[r * 8 + (t >> 5)] & ((1u << lane) - 1))] = (uint16_t)(r * 256 + t);
   }
+  __syncthreads();
+  if (c >= cols) return;
+  Col<VEC> old;
+  if (ACC) old = Col<VEC>::load(dtable + (int64_t)v * ld, c);
+  Col<VEC> acc = Col<VEC>::zero();
+  const float* at = dout + (int64_t)VEC * c;
+  int h = 0;
+  for (; h + FEW_U <= many; h += FEW_U) {  // sums of FEW_U rows, then of these
+    Col<VEC> x[FEW_U];
+#pragma unroll
+    for (int k = 0; k < FEW_U; ++k) x[k] = Col<VEC>::load(at + list[h + k] * ldo, 0);
+#pragma unroll
+    for (int k = 1; k < FEW_U; ++k) x[0].add(x[k]);
+    acc.add(x[0]);
+  }
+#pragma unroll 4
+  for (; h < many; ++h) acc.add(Col<VEC>::load(at + list[h] * ldo, 0));
   Col<VEC> r = acc.times(scale);
-  r.add(old);
+  if (ACC) r.add(old);
   r.store(dtable + (int64_t)v * ld, c);
 }
 
@@ -451,9 +525,10 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_place(const EmbedSort e, cons
 // takes no longer than many rare ones.  A run (the positions of one token) of at
 // most 2 T goes whole to the tile it starts in.  A longer one is cut at the
 // tiles' borders: what came in from the tile before is the tile's partial 0, the
-// start of what goes on its partial 1 (what does both, partial 0).  T is 64, or
-// 16 where 64 would leave SMs without a tile (65536 x 1024: 104 us with 64, 141 with
-// 16).  16384 x 4096 into 32000 rows written whole: 119 us, 6.6 TB/s.
+// start of what goes on its partial 1 (what does both, partial 0).  T is 64, or 32
+// or 16 where 64 would leave SMs without a tile (added: 65536 x 1024 104 us with 64,
+// 141 with 16; 4096 x 4096 39.3 and 42.6; 4147 x 3243 39.0 with 32, 42.3 with 16).
+// 16384 x 4096 into 32000 rows written whole: 119 us, 6.6 TB/s.
 struct EmbedSum {
   const float* dout;
   int64_t ldo, cols;
@@ -489,17 +564,8 @@ __device__ __forceinline__ void embed_zero(const EmbedSort& e, const EmbedSum& a
     const int k = e.key((int)(v0 + lane));
     gone = e.start[k] == e.start[k + 1];
   }
-  for (uint32_t some = __ballot_sync(0xffffffffu, gone); some; some &= some - 1) {
-    float* row = a.dtable + (v0 + __ffs(some) - 1) * a.ld;
-    int64_t head = (4 - (((uintptr_t)row >> 2) & 3)) & 3;
-    if (head > D) head = D;
-    const int64_t body = (D - head) >> 2;
-    if (lane < head) row[lane] = 0.0f;
-    float4* mid = reinterpret_cast<float4*>(row + head);
-#pragma unroll 4
-    for (int64_t q = lane; q < body; q += 32) mid[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (lane < D - head - 4 * body) row[head + 4 * body + lane] = 0.0f;
-  }
+  for (uint32_t some = __ballot_sync(0xffffffffu, gone); some; some &= some - 1)
+    clear_row(a.dtable + (v0 + __ffs(some) - 1) * a.ld, D, lane, 32);
 }
 
 // (4 CTAs to an SM with the old values in flight: 136 registers would leave 3, and
@@ -647,7 +713,11 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) k_embed_join(const EmbedSum a,
 }
 
 // ---- launches -----------------------------------------------------------------------------
-static bool aligned_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
+// the widest column that D and the rows of both buffers allow
+static int col_width(int64_t D, const void* p, int64_t ldp, const void* q, int64_t ldq) {
+  const int64_t all = D | ldp | ldq | (int64_t)((((uintptr_t)p | (uintptr_t)q) & 15) >> 2);
+  return all % 4 == 0 ? 4 : (all % 2 == 0 ? 2 : 1);
+}
 
 static unsigned grid_of(int64_t groups, int64_t chunks, const char* what) {
   TP_REQUIRE(groups <= INT_MAX / chunks, "%s: too many tokens, rows or columns for one launch", what);
@@ -657,10 +727,10 @@ static unsigned grid_of(int64_t groups, int64_t chunks, const char* what) {
 void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
                   float scale, float* out, int64_t ldo) {
   if (n == 0 || D == 0) return;
-  const bool vec = D % 4 == 0 && aligned_rows(table, ld) && aligned_rows(out, ldo);
-  const int64_t cols = vec ? D / 4 : D;
+  const int vec = col_width(D, table, ld, out, ldo);
+  const int64_t cols = D / vec;
   // columns of a thread; 20000 x 777 by 16 17.5 us, by 8 21.2; 200000 x 33 14.3 and 10.7
-  const int U = vec ? 4 : (cols > 512 ? 16 : 8);
+  const int U = vec == 4 ? 4 : (vec == 1 && cols > 512 ? 16 : 8);
   const int64_t need = (cols + U - 1) / U;  // threads
   const int chunks = (int)((need + LOOK_TX - 1) / LOOK_TX);
   int tx = block_cols(need);
@@ -670,7 +740,8 @@ void launch_embed(const float* table, int64_t ld, const void* ids, int kind, int
 #define TP_EMBED(VEC, U)                                                                                         \
   TP_LAUNCH((k_embed<VEC, U>), grid, dim3(tx, ty), 0, table, ld, ids, kind, n, (int)V, (uint32_t)cols, chunks, scale, \
             out, ldo)
-  if (vec) TP_EMBED(4, 4);
+  if (vec == 4) TP_EMBED(4, 4);
+  else if (vec == 2) TP_EMBED(2, 8);
   else if (U == 16) TP_EMBED(1, 16);
   else TP_EMBED(1, 8);
 #undef TP_EMBED
@@ -680,11 +751,12 @@ struct EmbedPlan {
   int64_t per, start, pos, tok, cut, count, first, spos, stok, partial, ldp, bytes, tiles, share;
   int g, T, B;
   bool split;
-  EmbedPlan(int64_t n, int64_t V, int64_t D) {
+  EmbedPlan(int64_t n, int64_t V, int64_t D) {  // n > 0
     g = 7;  // 128 CTAs for 148 SMs
     while (g < MOST_G && ((int64_t)SORT_TOKENS << g) < V) ++g;
     per = (V + (1 << g) - 1) >> g;
-    T = n / 64 * D >= 148 * 8 * 512 ? 64 : 16;  // 512 values of a row to a CTA, 8 CTAs to an SM
+    const int64_t work = n / 64 * D / 512;  // CTAs of 512 columns by 64 positions
+    T = work >= 148 * 4 ? 64 : (work >= 148 * 2 ? 32 : 16);
     tiles = (n + T - 1) / T;
     ldp = (D + 3) / 4 * 4;
     auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
@@ -695,7 +767,7 @@ struct EmbedPlan {
     // the whole gradient at a width of 64: 32768 ids of 32000 tokens 24.8 us in one
     // launch, 27.5 split first; 65536 ids 33.9 and 31.6
     split = per > SORT_TOKENS || n << g > (int64_t)1 << 22;
-    const int64_t words = n > 0 ? (n + 31) / 32 : 1;
+    const int64_t words = (n + 31) / 32;
     share = (words + 147) / 148;
     B = split ? (int)((words + share - 1) / share) : 0;
     count = cut + up(tiles * 8);
@@ -707,12 +779,12 @@ struct EmbedPlan {
   }
 };
 
-int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return EmbedPlan(n, V, D).bytes; }
+int64_t embed_bwd_ws(int64_t n, int64_t V, int64_t D) { return n <= EMB_FEW ? 0 : EmbedPlan(n, V, D).bytes; }
 
 template <int VEC, bool ACC>
 static void launch_sum(const EmbedSort& e, EmbedSum a, int64_t D) {
   const char* what = "token_embedding_backward";
-  a.cols = VEC == 4 ? D / 4 : D;
+  a.cols = D / VEC;
   const int tx = block_cols(a.cols), ty = EMB_NT / tx;
   a.chunks = (int)((a.cols + tx - 1) / tx);
   a.tile_ctas = (a.tiles + ty - 1) / ty;
@@ -721,7 +793,6 @@ static void launch_sum(const EmbedSort& e, EmbedSum a, int64_t D) {
   const int64_t grid = (int64_t)grid_of(a.tile_ctas, a.chunks, what) + zero_ctas;
   TP_REQUIRE(grid <= INT_MAX, "%s: too many tokens, rows or columns for one launch", what);
   TP_LAUNCH((k_embed_sum<VEC, ACC>), (unsigned)grid, dim3(tx, ty), 0, e, a);
-  if (a.tiles < 2) return;  // nothing is cut
   const int jchunks = (int)((D + 127) / 128);
   TP_LAUNCH(k_embed_join<ACC>, grid_of((a.tiles + JOIN_TILES - 1) / JOIN_TILES, jchunks, what), dim3(32, JOIN_ROWS), 0,
             a, D, jchunks);
@@ -740,13 +811,24 @@ static void raise_smem(K* kernel, int bytes) {
 void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind, int64_t n, int64_t V, int64_t D,
                       float scale, int64_t pad, bool accumulate, float* dtable, int64_t ld, void* ws) {
   if (D == 0 || (n == 0 && accumulate)) return;
-  const bool vec = D % 4 == 0 && aligned_rows(dout, ldo) && aligned_rows(dtable, ld);
-  if (accumulate && n <= EMB_FEW) {
-    const int64_t cols = vec ? D / 4 : D;
+  const int vec = col_width(D, dout, ldo, dtable, ld);
+  if (n <= EMB_FEW) {
+    const char* what = "token_embedding_backward";
+    const int64_t cols = D / vec;
     const int chunks = (int)((cols + 255) / 256);
-    const unsigned grid = grid_of(n, chunks, "token_embedding_backward");
-    if (vec) TP_LAUNCH(k_embed_few<4>, grid, 256, 0, dout, ldo, ids, kind, (int)n, V, cols, chunks, scale, pad, dtable, ld);
-    else TP_LAUNCH(k_embed_few<1>, grid, 256, 0, dout, ldo, ids, kind, (int)n, V, cols, chunks, scale, pad, dtable, ld);
+    const int clear = (int)(FEW_CLEAR_VALUES / D < 1 ? 1 : (FEW_CLEAR_VALUES / D < FEW_CLEAR ? FEW_CLEAR_VALUES / D : FEW_CLEAR));
+    const int64_t grid = (int64_t)grid_of(n, chunks, what) + (accumulate ? 0 : (V + clear - 1) / clear);
+    TP_REQUIRE(grid <= INT_MAX, "%s: too many tokens, rows or columns for one launch", what);
+#define TP_FEW(VEC, ACC)                                                                                          \
+  TP_LAUNCH((k_embed_few<VEC, ACC>), (unsigned)grid, 256, 0, dout, ldo, ids, kind, (int)n, V, cols, chunks, scale, pad, \
+            dtable, ld, clear)
+    if (accumulate && vec == 4) TP_FEW(4, true);
+    else if (accumulate && vec == 2) TP_FEW(2, true);
+    else if (accumulate) TP_FEW(1, true);
+    else if (vec == 4) TP_FEW(4, false);
+    else if (vec == 2) TP_FEW(2, false);
+    else TP_FEW(1, false);
+#undef TP_FEW
     return;
   }
   const EmbedPlan p(n, V, D);
@@ -796,9 +878,11 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   a.partial = (float*)(base + p.partial);
   a.ldp = p.ldp;
   a.cut = (int2*)(base + p.cut);
-  if (vec && accumulate) launch_sum<4, true>(e, a, D);
-  else if (vec) launch_sum<4, false>(e, a, D);
+  if (accumulate && vec == 4) launch_sum<4, true>(e, a, D);
+  else if (accumulate && vec == 2) launch_sum<2, true>(e, a, D);
   else if (accumulate) launch_sum<1, true>(e, a, D);
+  else if (vec == 4) launch_sum<4, false>(e, a, D);
+  else if (vec == 2) launch_sum<2, false>(e, a, D);
   else launch_sum<1, false>(e, a, D);
 }
 
