@@ -211,6 +211,7 @@ constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a threa
 constexpr int SORT_WORDS = 8192;          // positions / 32 whose hits are kept in shared memory
 constexpr int SORT_LIST = 768;            // hits that a warp lists before it places them
 constexpr int MOST_G = 10;                // log2 of the most CTAs
+constexpr int PLACE_U = 4;                // ids of a thread in flight as an owner places its own
 constexpr int SORT_U = 16;                // ids of a thread in flight, and words listed at once
 
 struct EmbedSort {
@@ -502,20 +503,25 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_place(const EmbedSort e, cons
     }
     __syncthreads();
     base = embed_places(e, sort_sm, me, l0, W, base, sh);
-    int v = i0 + lane < i1 ? p.tok[i0 + lane] : -1, at = v >= 0 ? p.pos[i0 + lane] : 0;
-    for (int64_t i = i0; i < i1; i += 32) {
-      const bool more = i + 32 + lane < i1;
-      const int nv = more ? p.tok[i + 32 + lane] : -1, nat = more ? p.pos[i + 32 + lane] : 0;
-      const bool take = v >= 0 && (uint32_t)local(v) < (uint32_t)W;
-      const uint32_t some = __ballot_sync(0xffffffffu, take);
-      if (take) {
-        const int to = embed_take(some, v, &mine[local(v)]);
-        e.pos[to] = at;
-        e.tok[to] = v;
+    for (int64_t i = i0; i < i1; i += 32 * PLACE_U) {
+      int v[PLACE_U], at[PLACE_U];
+#pragma unroll
+      for (int q = 0; q < PLACE_U; ++q) {
+        const int64_t j = i + 32 * q + lane;
+        v[q] = j < i1 ? p.tok[j] : -1;
+        at[q] = j < i1 ? p.pos[j] : 0;
       }
-      __syncwarp();
-      v = nv;
-      at = nat;
+#pragma unroll
+      for (int q = 0; q < PLACE_U; ++q) {
+        const bool take = v[q] >= 0 && (uint32_t)local(v[q]) < (uint32_t)W;
+        const uint32_t some = __ballot_sync(0xffffffffu, take);
+        if (take) {
+          const int to = embed_take(some, v[q], &mine[local(v[q])]);
+          e.pos[to] = at[q];
+          e.tok[to] = v[q];
+        }
+        __syncwarp();
+      }
     }
     __syncthreads();
   }
@@ -526,8 +532,8 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_place(const EmbedSort e, cons
 // most 2 T goes whole to the tile it starts in.  A longer one is cut at the
 // tiles' borders: what came in from the tile before is the tile's partial 0, the
 // start of what goes on its partial 1 (what does both, partial 0).  T is 64, or 32
-// or 16 where 64 would leave SMs without a tile (added: 65536 x 1024 104 us with 64,
-// 141 with 16; 4096 x 4096 39.3 and 42.6; 4147 x 3243 39.0 with 32, 42.3 with 16).
+// or 16 where 64 would leave SMs without a tile (added: 65536 x 1024 98 us with 64,
+// 105 with 24; 4096 x 4096 39.3, 42.6 with 16; 4147 x 3243 39.0 with 32, 42.3 with 16).
 // 16384 x 4096 into 32000 rows written whole: 119 us, 6.6 TB/s.
 struct EmbedSum {
   const float* dout;
@@ -568,8 +574,8 @@ __device__ __forceinline__ void embed_zero(const EmbedSort& e, const EmbedSum& a
     clear_row(a.dtable + (v0 + __ffs(some) - 1) * a.ld, D, lane, 32);
 }
 
-// (4 CTAs to an SM with the old values in flight: 136 registers would leave 3, and
-// 65536 x 1024 then takes 116 us instead of 104; 8 would spill, 181 us.)
+// (4 CTAs to an SM with the old values in flight: its registers would leave 3, and
+// 131622 x 332 added then takes 94.5 us instead of 87.4; 8 would spill.)
 template <int VEC, bool ACC>
 __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(const EmbedSort e, const EmbedSum a) {
   ::tp::pdl_enter();
@@ -621,10 +627,16 @@ __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(c
     }
   };
   // eight positions at a time, on eight-position boundaries (one past the last is
-  // still inside the workspace); lo, hi: which of them are the tile's
+  // still inside the workspace), those of the next batch fetched ahead (65536 x 1024
+  // added: 98 us, 104 without); lo, hi: which of them are the tile's
+  int4 nt0, nt1, np0, np1;
+  auto fetch = [&](int s) {
+    nt0 = *reinterpret_cast<const int4*>(e.tok + s), nt1 = *reinterpret_cast<const int4*>(e.tok + s + 4);
+    np0 = *reinterpret_cast<const int4*>(e.pos + s), np1 = *reinterpret_cast<const int4*>(e.pos + s + 4);
+  };
   auto batch = [&](int s, int lo, int hi) {
-    const int4 t0 = *reinterpret_cast<const int4*>(e.tok + s), t1 = *reinterpret_cast<const int4*>(e.tok + s + 4);
-    const int4 p0 = *reinterpret_cast<const int4*>(e.pos + s), p1 = *reinterpret_cast<const int4*>(e.pos + s + 4);
+    const int4 t0 = nt0, t1 = nt1, p0 = np0, p1 = np1;
+    if (s + SUM_U < s1) fetch(s + SUM_U);
     const int tok[SUM_U] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
     const int pos[SUM_U] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
     Col<VEC> x[SUM_U], old[ACC ? SUM_U : 1];
@@ -651,6 +663,7 @@ __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(c
       }
   };
   int s = from & ~(SUM_U - 1);
+  fetch(s);
   if (s < from) {
     batch(s, from - s, s1 - s < SUM_U ? s1 - s : SUM_U);
     s += SUM_U;
@@ -667,19 +680,19 @@ __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(c
 }
 
 // The runs that were cut: the tile one starts in adds up its partial 1 and the
-// partials 0 of the tiles after it, in f64: eight threads take every eighth,
-// and their sums are added in order.  A CTA looks through 8 tiles for such starts
-// (16384 x 4096: 7 us; through 32: 11).
-constexpr int JOIN_TILES = 8, JOIN_ROWS = 8;
+// partials 0 of the tiles after it, in f64: a CTA is `across` threads wide, its
+// rows of threads take every so many-th tile, and their sums meet pair by pair.  A
+// CTA looks through 8 tiles for such starts (16384 x 4096: 7 us; through 32: 11).
+constexpr int JOIN_TILES = 8, JOIN_NT = 256;
 
 template <bool ACC>
-__global__ void __launch_bounds__(32 * JOIN_ROWS) k_embed_join(const EmbedSum a, int64_t D, int chunks) {
+__global__ void __launch_bounds__(JOIN_NT) k_embed_join(const EmbedSum a, int64_t D, int chunks, int across) {
   ::tp::pdl_enter();
-  __shared__ double sh[JOIN_ROWS][4][32];
-  const int lane = threadIdx.x, r = threadIdx.y;
+  __shared__ double sh[4][JOIN_NT];
+  const int t = threadIdx.x, lane = t & 31, r = t / across, rows = JOIN_NT / across;
   const int64_t group = blockIdx.x / chunks;
-  const int64_t c4 = (int64_t)(blockIdx.x - group * chunks) * 32 + lane;  // a 4-value column of the partials
-  const int64_t mine = group * JOIN_TILES + lane;                         // every warp looks at the same tiles
+  const int64_t c4 = (int64_t)(blockIdx.x - group * chunks) * across + t - r * across;  // a 4-value column of the partials
+  const int64_t mine = group * JOIN_TILES + lane;                                 // every warp looks at the same tiles
   const int2 run = lane < JOIN_TILES && mine < a.tiles ? a.cut[mine] : make_int2(-1, 0);
   for (uint32_t some = __ballot_sync(0xffffffffu, run.x >= 0); some; some &= some - 1) {
     const int which = __ffs(some) - 1;
@@ -695,18 +708,28 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) k_embed_join(const EmbedSum a,
     };
     if (4 * c4 < D) {
       if (r == 0) add(2 * tile + 1);
-#pragma unroll 4
-      for (int64_t k = tile + 1 + r; k <= last; k += JOIN_ROWS) add(2 * k);
+#pragma unroll 8
+      for (int64_t k = tile + 1 + r; k <= last; k += rows) add(2 * k);
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sh[r][q][lane] = acc[q];
+    for (int q = 0; q < 4; ++q) sh[q][t] = acc[q];
     __syncthreads();
-    if (r < 4) {  // warp r: value r of each column
-      double sum = 0.0;
-      for (int i = 0; i < JOIN_ROWS; ++i) sum += sh[i][r][lane];
-      const float g = (float)(sum * a.scale);
-      float* row = a.dtable + (int64_t)v * a.ld + 4 * c4 + r;
-      if (4 * c4 + r < D) *row = ACC ? *row + g : g;
+    int o = rows / 2;
+    while (o >= last - tile) o >>= 1;  // rows from last - tile on have nothing
+    for (; o > 0; o >>= 1) {
+      if (r < o)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sh[q][t] += sh[q][t + o * across];
+      __syncthreads();
+    }
+    if (r == 0) {
+      float* row = a.dtable + (int64_t)v * a.ld + 4 * c4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (4 * c4 + q < D) {
+          const float g = (float)(sh[q][t] * a.scale);
+          row[q] = ACC ? row[q] + g : g;
+        }
     }
     __syncthreads();
   }
@@ -793,9 +816,11 @@ static void launch_sum(const EmbedSort& e, EmbedSum a, int64_t D) {
   const int64_t grid = (int64_t)grid_of(a.tile_ctas, a.chunks, what) + zero_ctas;
   TP_REQUIRE(grid <= INT_MAX, "%s: too many tokens, rows or columns for one launch", what);
   TP_LAUNCH((k_embed_sum<VEC, ACC>), (unsigned)grid, dim3(tx, ty), 0, e, a);
-  const int jchunks = (int)((D + 127) / 128);
-  TP_LAUNCH(k_embed_join<ACC>, grid_of((a.tiles + JOIN_TILES - 1) / JOIN_TILES, jchunks, what), dim3(32, JOIN_ROWS), 0,
-            a, D, jchunks);
+  int across = 1;
+  while (across < 32 && 4 * across < D) across *= 2;
+  const int jchunks = (int)((D + 4 * across - 1) / (4 * across));
+  TP_LAUNCH(k_embed_join<ACC>, grid_of((a.tiles + JOIN_TILES - 1) / JOIN_TILES, jchunks, what), JOIN_NT, 0, a, D,
+            jchunks, across);
 }
 
 // Lets a kernel have that much dynamic shared memory; asked for once per kernel.
