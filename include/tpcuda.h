@@ -489,9 +489,9 @@ TP_API int tpk_token_logprobs_backward(const float* logits, int64_t ld, const vo
 TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, int ids_kind, int64_t n,
                                int64_t vocab, int64_t dim, float scale, float* out, int64_t ldo);
 /* accumulate 0 writes every row of dtable, 1 adds to the rows of present
- * tokens.  ws: at least the bytes that tpk_token_embedding_backward_ws names,
- * used from the call's first kernel to its last; calls whose work may overlap
- * on the GPU need one each. */
+ * tokens.  ws: at least the bytes that tpk_token_embedding_backward_ws names
+ * (0 for up to 512 tokens: ws may be NULL), used from the call's first kernel to
+ * its last; calls whose work may overlap on the GPU need one each. */
 TP_API int tpk_token_embedding_backward_ws(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes);
 TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const void* ids, int ids_kind, int64_t n,
                                         int64_t vocab, int64_t dim, float scale, int64_t padding_id, int accumulate,

@@ -121,6 +121,35 @@ def test_gradient_patterns(cuda_rt, n, what, accumulate):
         assert np.array_equal(got, old if accumulate else np.zeros((V, D)))
 
 
+@pytest.mark.parametrize("D, ld, ldo, offset", [(1, 0, 0, 0), (2, 0, 0, 8), (6, 2, 4, 0), (30, 0, 2, 8), (31, 0, 1, 4),
+                                                 (34, 0, 0, 0), (500, 2, 0, 8), (521, 3, 7, 12), (1026, 0, 0, 0),
+                                                 (1024, 4, 8, 0), (1024, 1, 0, 0), (9001, 0, 0, 0)])
+def test_widths_and_strides(cuda_rt, D, ld, ldo, offset):
+    """Columns of 4, 8 and 16 bytes, by the widest that both buffers allow; around
+    the most tokens that take one launch."""
+    rng = np.random.default_rng(D)
+    for n, V in ((0, 9), (1, 70), (512, 3), (512, 1500), (513, 70)):
+        ids = rng.integers(-1, V + 1, n)
+        dout = rng.standard_normal((n, D)).astype(np.float32)
+        table = rng.standard_normal((V, D)).astype(np.float32)
+        check_grad(cuda_rt, dout, ids, V, 0.75, pad=V // 2, kind=n % 2, ld=ld, ldo=ldo, offset=offset)
+        check_grad(cuda_rt, dout, ids, V, 0.75, old=table, kind=n % 2, ld=ld, ldo=ldo, offset=offset)
+        if n:
+            got = lookup(cuda_rt, table, ids, 0.75, kind=n % 2, ld=ld, ldo=ldo, offset=offset)
+            want = np.full((n, D), np.nan, np.float32)
+            keep = (ids >= 0) & (ids < V)
+            want[keep] = table[ids[keep]] * np.float32(0.75)
+            assert np.array_equal(got, want, equal_nan=True)
+
+
+def test_gradient_of_few_tokens_needs_no_workspace(cuda_rt):
+    rt = cuda_rt
+    G, I = Buf(rt, np.ones((4, 8), np.float32)), Buf(rt, np.array([2, 0, 2, 7], np.int32))
+    T = Buf(rt, np.full((5, 8), GUARD, np.float32))
+    assert rt.lib.tpk_token_embedding_backward(G.ptr, 8, I.ptr, 1, 4, 5, 8, 1.0, -1, 0, T.ptr, 8, None, 0) == 0
+    assert np.array_equal(T.read(), np.array([1, 0, 2, 0, 0], np.float32)[:, None] * np.ones(8, np.float32))
+
+
 def test_gradient_of_long_sums(cuda_rt):
     """One token in 70000 of 100000 positions: the bound grows with the sums'
     length as far as two levels of 256 go."""

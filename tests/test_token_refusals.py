@@ -85,6 +85,8 @@ def test_embedding_backward(lib, change, word):
 def test_embedding_workspace(lib):
     b = ctypes.c_int64(-1)
     assert lib.tpk_token_embedding_backward_ws(16384, 32000, 4096, ctypes.byref(b)) == 0 and b.value > 0
+    assert lib.tpk_token_embedding_backward_ws(513, 10, 8, ctypes.byref(b)) == 0 and b.value > 0
+    assert lib.tpk_token_embedding_backward_ws(512, 32000, 4096, ctypes.byref(b)) == 0 and b.value == 0
     refused(lib, lib.tpk_token_embedding_backward_ws(-1, 10, 8, ctypes.byref(b)), "tokens")
     refused(lib, lib.tpk_token_embedding_backward_ws(1, 0, 8, ctypes.byref(b)), "vocabulary")
     refused(lib, lib.tpk_token_embedding_backward_ws(1, 10, 8, None), "bytes")
