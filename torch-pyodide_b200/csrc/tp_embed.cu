@@ -103,9 +103,10 @@ __device__ __forceinline__ void clear_row(float* row, int64_t D, int t, int n) {
 // One CTA per (position, 256 columns), which compares its token with all ids at
 // once: the first position of a token sums all of them, in order.  Reads the ids
 // n times over, and a frequent token's rows by one thread per column: 256 x 1024
-// takes 5.2 us against 14.1 sorted, 1024 x 4096 23.6 against 22.5, 512 x 1024 all of
-// one token 39.  Where rows are written, not added to, more CTAs clear `clear` rows
-// each that no id names (2 x 2846 into 3946 rows: 7.8 us, 35 sorted).
+// takes 5.2 us against 14.1 sorted, 1024 x 1024 7.2 against 16.9, but all of one
+// token 77 against 16 (512 of them: 39), hence the bound.  Where rows are written,
+// not added to, more CTAs clear `clear` rows each that no id names (2 x 2846 into
+// 3946 rows: 7.8 us, 35 sorted).
 constexpr int EMB_FEW = 512;
 constexpr int FEW_U = 16;  // rows in flight (500 x 4096 of 10 tokens, added: 11.4 us, 14.4 with 8)
 constexpr int FEW_CLEAR = 1024;       // rows that a CTA looks at, at most
