@@ -93,10 +93,35 @@ struct LpStat {
     S *= s;
     m = M;
   }
-  __device__ __forceinline__ void add(float x) {
-    const float y = fmaxf(x - m, LP_FLOOR), e = lp_exp(y);
-    S += e;
-    T = fmaf(e, y, T);
+};
+
+// A thread's running statistics, 16 logits at a time.  Once the maximum's 1 is in
+// S, a term below half a step of it, 2^-24, would be lost, and with it the thread's
+// share of a tail that far down.  So 16 exponentials are summed among themselves,
+// and what their sum loses on its way into S goes into the next one (Kahan's
+// compensation): two roundings, however long the row is.  The maximum adds 0 to T,
+// whose 16 terms are summed among themselves too.  (8192 x 131072: 588 us, one by
+// one 585; 1999 x 50021 with 5 alternatives: 71.5, 70.6.)
+struct LpRun : LpStat {
+  float lost;  // of S
+  __device__ __forceinline__ void move(float M) {
+    lost *= lp_exp(fmaxf(m - M, LP_FLOOR));
+    LpStat::move(M);
+  }
+  __device__ __forceinline__ void add(const float4 (&v)[4]) {
+    float s[4], t[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float y0 = fmaxf(v[q].x - m, LP_FLOOR), y1 = fmaxf(v[q].y - m, LP_FLOOR);
+      const float y2 = fmaxf(v[q].z - m, LP_FLOOR), y3 = fmaxf(v[q].w - m, LP_FLOOR);
+      const float e0 = lp_exp(y0), e1 = lp_exp(y1), e2 = lp_exp(y2), e3 = lp_exp(y3);
+      s[q] = (e0 + e1) + (e2 + e3);
+      t[q] = fmaf(e3, y3, fmaf(e2, y2, fmaf(e1, y1, e0 * y0)));
+    }
+    const float more = ((s[0] + s[1]) + (s[2] + s[3])) - lost, sum = S + more;
+    lost = (sum - S) - more;
+    S = sum;
+    T += (t[0] + t[1]) + (t[2] + t[3]);
   }
 };
 
@@ -173,8 +198,14 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
   float tau = s.m;
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) s.m = lp_max(s.m, __shfl_xor_sync(ALL, s.m, o));
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of S: see LpRun
 #pragma unroll
-  for (int k = 0; k < 4 * N; ++k) s.add(v[k]);
+  for (int k = 0; k < 4 * N; ++k) {
+    const float y = fmaxf(v[k] - s.m, LP_FLOOR), e = lp_exp(y);
+    part[k & 3] += e;
+    s.T = fmaf(e, y, s.T);
+  }
+  s.S = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) {
     s.S += __shfl_xor_sync(ALL, s.S, o);
@@ -582,7 +613,9 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
   const int64_t lo = per * part < V ? per * part : V, hi = lo + per < V ? lo + per : V;
   const LpPart<NT> p(xr, lo, hi);
   const int batches = p.batches();
-  LpStat s{-INFINITY, 0.0f, 0.0f};
+  LpRun run;
+  run.m = -INFINITY;
+  run.S = run.T = run.lost = 0.0f;
   LpUnit unit[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) unit[q] = LpUnit{-INFINITY, -INFINITY, 0};
@@ -608,19 +641,14 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT)
       }
       m = lp_max(lp_max(unit[0].m, unit[1].m), lp_max(unit[2].m, unit[3].m));
     } else {
-      m = s.m;
+      m = run.m;
 #pragma unroll
       for (int q = 0; q < 4; ++q) m = lp_max(m, lp_max(lp_max(v[q].x, v[q].y), lp_max(v[q].z, v[q].w)));
     }
-    if (m != s.m) s.move(m);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s.add(v[q].x);
-      s.add(v[q].y);
-      s.add(v[q].z);
-      s.add(v[q].w);
-    }
+    if (m != run.m) run.move(m);
+    run.add(v);
   }
+  LpStat s = run;
   float own = s.m;
   const float most = lp_warp_max(own);
   s.move(most);
