@@ -471,7 +471,8 @@ TP_API int tp_token_embedding(int64_t table, int64_t ids, float scale, tp_handle
  * positions whose id is v, in an order fixed by the positions (equal inputs,
  * equal bits); ids equal to padding_id (-1: none) or outside [0, vocab) are
  * left out.  into 0: a new [vocab, dim] tensor; else added to that tensor's rows
- * in place (rows of absent tokens are not touched), which *out then names. */
+ * in place (rows of absent tokens are not touched), which *out then names.  At
+ * most 2^31 - 2^11 positions. */
 TP_API int tp_token_embedding_backward(int64_t grad_out, int64_t ids, int64_t vocab, float scale, int64_t padding_id,
                                        int64_t into, tp_handle* out);
 /* The same on device pointers: rows of `ld` (ldd, ldo) values, of which the

@@ -912,8 +912,13 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
   else launch_sum<1, false>(e, a, D);
 }
 
-static void check_embed(int64_t n, int64_t V, int64_t D, int64_t ld, int64_t ldo, const char* what) {
-  TP_REQUIRE(n >= 0 && n < INT_MAX, "%s: %lld tokens is outside [0, 2^31 - 1)", what, (long long)n);
+// Most positions: the gradient's kernels round them up to SORT_NT (a share of a
+// warp) and to SUM_U (a batch) in 32 bits.
+constexpr int64_t LOOK_MOST = INT_MAX - 1, EMB_MOST = ((int64_t)1 << 31) - 2048;
+static_assert(EMB_MOST + SORT_NT <= INT_MAX && EMB_MOST + SUM_U <= INT_MAX, "positions are rounded up in 32 bits");
+
+static void check_embed(int64_t n, int64_t most, int64_t V, int64_t D, int64_t ld, int64_t ldo, const char* what) {
+  TP_REQUIRE(n >= 0 && n <= most, "%s: %lld tokens is outside [0, %lld]", what, (long long)n, (long long)most);
   check_vocab(V, what);
   TP_REQUIRE(D >= 0 && D <= INT_MAX, "%s: a width of %lld is outside [0, 2^31)", what, (long long)D);
   TP_REQUIRE(ld >= D && ldo >= D, "%s: a row stride (%lld, %lld) is shorter than the width %lld", what, (long long)ld,
@@ -930,7 +935,7 @@ TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, 
                                int64_t vocab, int64_t dim, float scale, float* out, int64_t ldo) {
   return guard([&] {
     const char* what = "token_embedding";
-    check_embed(n, vocab, dim, ld, ldo, what);
+    check_embed(n, LOOK_MOST, vocab, dim, ld, ldo, what);
     check_ids_kind(ids_kind, what);
     if (n == 0 || dim == 0) return;
     TP_REQUIRE(table && ids && out, "%s: table, ids and out must not be NULL", what);
@@ -942,7 +947,7 @@ TP_API int tpk_token_embedding(const float* table, int64_t ld, const void* ids, 
 
 TP_API int tpk_token_embedding_backward_ws(int64_t n, int64_t vocab, int64_t dim, int64_t* bytes) {
   return guard([&] {
-    check_embed(n, vocab, dim, dim, dim, "token_embedding_backward_ws");
+    check_embed(n, EMB_MOST, vocab, dim, dim, dim, "token_embedding_backward_ws");
     TP_REQUIRE(bytes, "token_embedding_backward_ws: bytes is NULL");
     *bytes = embed_bwd_ws(n, vocab, dim);
   });
@@ -953,7 +958,7 @@ TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const vo
                                         float* dtable, int64_t ld, void* ws, int64_t ws_bytes) {
   return guard([&] {
     const char* what = "token_embedding_backward";
-    check_embed(n, vocab, dim, ld, ldo, what);
+    check_embed(n, EMB_MOST, vocab, dim, ld, ldo, what);
     check_ids_kind(ids_kind, what);
     TP_REQUIRE(padding_id >= -1 && padding_id < vocab, "%s: padding_id %lld is neither -1 nor a row of the table",
                what, (long long)padding_id);
@@ -976,7 +981,7 @@ TP_API int tp_token_embedding(int64_t table, int64_t ids, float scale, tp_handle
     const Tensor T = get(table), I = get(ids);
     TP_REQUIRE(T.ndim == 2 && T.phys == PHYS_F32, "%s: expects a float table [vocab, dim]", what);
     TP_REQUIRE(I.ndim < TP_MAX_DIMS, "%s: ids of rank %d leave no dim for the rows", what, I.ndim);
-    check_embed(I.numel, T.shape[0], T.shape[1], T.shape[1], T.shape[1], what);
+    check_embed(I.numel, LOOK_MOST, T.shape[0], T.shape[1], T.shape[1], T.shape[1], what);
     std::vector<int64_t> s = shape_of(I);
     s.push_back(T.shape[1]);
     Outputs o;
@@ -995,7 +1000,7 @@ TP_API int tp_token_embedding_backward(int64_t grad_out, int64_t ids, int64_t vo
     const int64_t n = I.numel, D = G.shape[G.ndim - 1];
     TP_REQUIRE(n * D == G.numel, "%s: %lld token ids for a gradient of %lld values in rows of %lld", what,
                (long long)n, (long long)G.numel, (long long)D);
-    check_embed(n, vocab, D, D, D, what);
+    check_embed(n, EMB_MOST, vocab, D, D, D, what);
     TP_REQUIRE(padding_id >= -1 && padding_id < vocab, "%s: padding_id %lld is neither -1 nor a row of the table",
                what, (long long)padding_id);
     const Tensor T = into ? get(into) : Tensor();
