@@ -208,10 +208,13 @@ __global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dou
 // are n D 4 bytes from HBM.)
 constexpr int SORT_NT = 1024;
 constexpr int SORT_WARPS = SORT_NT / 32;
+constexpr int LEAST_G = 7, MOST_G = 10;   // log2 of the CTAs: 128 for 148 SMs, or more
 constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a thread each in the scan)
-constexpr int SORT_WORDS = 8192;          // positions / 32 whose hits are kept in shared memory
+constexpr int SORT_WORDS = 1024;          // positions / 32 of one launch: their hits are kept in shared memory
+constexpr int64_t SORT_READS = (int64_t)1 << 22;  // ids that the CTAs of one launch read in all, at most
+static_assert((SORT_READS >> LEAST_G) <= 32 * SORT_WORDS, "more positions than hits are kept of");
+static_assert(32 * SORT_WORDS <= 65536, "a list holds offsets of 16 bits");
 constexpr int SORT_LIST = 768;            // hits that a warp lists before it places them
-constexpr int MOST_G = 10;                // log2 of the most CTAs
 constexpr int PLACE_U = 4;                // ids of a thread in flight as an owner places its own
 constexpr int SORT_U = 16;                // ids of a thread in flight, and words listed at once
 
@@ -288,21 +291,20 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   int32_t* count = sort_sm;                                  // [warps][W]
   uint16_t* hits = (uint16_t*)(sort_sm + SORT_WARPS * W);    // [warps][SORT_LIST]
   uint32_t* words = (uint32_t*)(hits + SORT_WARPS * SORT_LIST);   // hits of 32 positions each
-  const int64_t nwords = (e.n + 31) >> 5;
-  const bool kept = nwords <= SORT_WORDS;
-  const int64_t per = (nwords + SORT_WARPS - 1) / SORT_WARPS;  // words of one warp: neighbours, so that order is kept
-  const int64_t w0 = per * w < nwords ? per * w : nwords, w1 = w0 + per < nwords ? w0 + per : nwords;
+  const int n = (int)e.n, nwords = (n + 31) >> 5;  // at most SORT_WORDS
+  const int per = (nwords + SORT_WARPS - 1) / SORT_WARPS;  // words of one warp: neighbours, so that order is kept
+  const int w0 = per * w < nwords ? per * w : nwords, w1 = w0 + per < nwords ? w0 + per : nwords;
   for (int i = t; i < SORT_WARPS * W; i += SORT_NT) count[i] = 0;
   __syncthreads();
-  auto token = [&](int64_t word) {
-    const int64_t p = word * 32 + lane;
-    return word < w1 && p < e.n ? token_id(e.ids, KIND, p) : -1;
+  auto token = [&](int word) {
+    const int p = word * 32 + lane;
+    return word < w1 && p < n ? token_id(e.ids, KIND, p) : -1;
   };
   int less = 0;
-  for (int64_t i = w0; i < w1; i += SORT_U) {
+  for (int i = w0; i < w1; i += SORT_U) {
     int v[SORT_U];
     uint32_t mine = 0u;
-    if (i + SORT_U <= w1 && (i + SORT_U) * 32 <= e.n) {
+    if (i + SORT_U <= w1 && (i + SORT_U) * 32 <= n) {
       const int32_t* at = static_cast<const int32_t*>(e.ids) + i * 32 + lane;  // either storage is 4 bytes
 #pragma unroll
       for (int q = 0; q < SORT_U; ++q) v[q] = token_id(at + 32 * q, KIND, 0);
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
       if (hit) atomicAdd(&count[w * W + e.local(v[q])], 1);
       mine = lane == q ? b : mine;
     }
-    if (kept && lane < SORT_U && i + lane < w1) words[i + lane] = mine;
+    if (lane < SORT_U && i + lane < w1) words[i + lane] = mine;
   }
   for (int o = 16; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
   if (lane == 0) sh[w] = less;
@@ -332,18 +334,9 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
   // lane each, the tokens of the next 32 under way.
   uint16_t* list = hits + SORT_LIST * w;
   int have = 0;
-  int64_t list0 = w0;  // the word that offsets count from
-  for (int64_t i = w0; i < w1; i += SORT_U) {
-    uint32_t mine = 0u;
-    if (kept) {
-      if (lane < SORT_U && i + lane < w1) mine = words[i + lane];
-    } else {
-      for (int j = 0; j < SORT_U; ++j) {
-        const int v = token(i + j);
-        const uint32_t b = __ballot_sync(0xffffffffu, e.valid(v) && e.owner(v) == me);
-        if (lane == j) mine = b;
-      }
-    }
+  int list0 = w0;  // the word that offsets count from
+  for (int i = w0; i < w1; i += SORT_U) {
+    uint32_t mine = lane < SORT_U && i + lane < w1 ? words[i + lane] : 0u;
     int at = __popc(mine);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -354,17 +347,17 @@ __global__ void __launch_bounds__(SORT_NT) k_embed_sort(const EmbedSort e) {
     at += have - __popc(mine);
     for (; mine; mine &= mine - 1) list[at++] = (uint16_t)(32 * (i - list0 + lane) + __ffs(mine) - 1);
     have += more;
-    // room for 16 words more, offsets of them within 16 bits, or the end
-    if (have <= SORT_LIST - 32 * SORT_U && i + 2 * SORT_U - list0 <= 2048 && i + SORT_U < w1) continue;
+    // room for 16 words more, or the end
+    if (have <= SORT_LIST - 32 * SORT_U && i + SORT_U < w1) continue;
     __syncwarp();
-    const int64_t first = list0 * 32;
+    const int first = list0 * 32;
     auto fetch = [&](int h) { return h < have ? token_id(e.ids, KIND, first + list[h]) : 0; };
     int v = fetch(lane);
     for (int h = 0; h < have; h += 32) {
       const int next = fetch(h + 32 + lane), k = have - h < 32 ? have - h : 32;
       if (lane < k) {
         const int to = embed_take(k == 32 ? 0xffffffffu : (1u << k) - 1, v, &count[w * W + e.local(v)]);
-        e.pos[to] = (int32_t)(first + list[h + lane]);
+        e.pos[to] = first + list[h + lane];
         e.tok[to] = v;
       }
       __syncwarp();
@@ -776,7 +769,7 @@ struct EmbedPlan {
   int g, T, B;
   bool split;
   EmbedPlan(int64_t n, int64_t V, int64_t D) {  // n > 0
-    g = 7;  // 128 CTAs for 148 SMs
+    g = LEAST_G;
     while (g < MOST_G && ((int64_t)SORT_TOKENS << g) < V) ++g;
     per = (V + (1 << g) - 1) >> g;
     const int64_t work = n / 64 * D / 512;  // CTAs of 512 columns by 64 positions
@@ -790,7 +783,7 @@ struct EmbedPlan {
     cut = tok + up(n * 4 + 32);
     // the whole gradient at a width of 64: 32768 ids of 32000 tokens 24.8 us in one
     // launch, 27.5 split first; 65536 ids 33.9 and 31.6
-    split = per > SORT_TOKENS || n << g > (int64_t)1 << 22;
+    split = per > SORT_TOKENS || n << g > SORT_READS;
     const int64_t words = (n + 31) / 32;
     share = (words + 147) / 148;
     B = split ? (int)((words + share - 1) / share) : 0;
@@ -885,10 +878,10 @@ void launch_embed_bwd(const float* dout, int64_t ldo, const void* ids, int kind,
     const int64_t W = p.per < SORT_TOKENS ? p.per : SORT_TOKENS;
     TP_LAUNCH(k_embed_place, 1u << p.g, SORT_NT, (size_t)SORT_WARPS * 4 * W, e, s);
   } else {
-    // at most 128 KB of counts, 48 of listed hits, 32 of hits
+    // at most 128 KB of counts, 48 of listed hits, 4 of hits
     const int most = (SORT_WARPS * (SORT_TOKENS + SORT_LIST / 2) + SORT_WORDS) * 4;
     const int64_t words = (n + 31) / 32;
-    const size_t smem = (size_t)(SORT_WARPS * (p.per + SORT_LIST / 2) + (words <= SORT_WORDS ? words : 0)) * 4;
+    const size_t smem = (size_t)(SORT_WARPS * (p.per + SORT_LIST / 2) + words) * 4;
     raise_smem(k_embed_sort<IDS_I32>, most);
     raise_smem(k_embed_sort<IDS_F32>, most);
     TP_LAUNCH(i32 ? k_embed_sort<IDS_I32> : k_embed_sort<IDS_F32>, 1u << p.g, SORT_NT, smem, e);
