@@ -776,6 +776,9 @@ struct LpGrad {
 // Rows of at most 1024 logits: a group of L lanes each, in 16-byte vectors where
 // the row of x and the row of dx start at the same offset from a boundary.
 // (65536 x 258: 30.0 us by 8 lanes, 38.7 by 32; x 1000: 90 and 80.)
+// A row without an upstream gradient is read no further than its lanes' first 16
+// values, which are fetched before that is known: 65536 x 1000, 90% ignored, 64.8
+// us (49.4 if it were known first, but 81.8 instead of 79.9 with none ignored).
 template <int L>
 __global__ void __launch_bounds__(128) k_logprobs_bwd_short(const float* x, int64_t ld, const void* __restrict__ ids,
                                                             int kind, const float* __restrict__ stats,
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(128) k_logprobs_bwd_short(const float* x, int6
     load(l);  // under way while the row's coefficients are fetched
     const LpGrad g(row, V, ids, kind, stats, entropy, dlogp, dentropy);
     for (int j = l; 4 * j < end; j += 4 * L) {
-      if (j > l) load(j);
+      if (j > l && !g.zero) load(j);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int u = 4 * (j + L * q), i = u - a;
@@ -824,7 +827,7 @@ __global__ void __launch_bounds__(128) k_logprobs_bwd_short(const float* x, int6
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (i + L * k < V) v[k] = xr[i + L * k];
+        if (i + L * k < V && !g.zero) v[k] = xr[i + L * k];
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (i + L * k < V) dr[i + L * k] = g.zero ? 0.0f : g(v[k], i + L * k);
