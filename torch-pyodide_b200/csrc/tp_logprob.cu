@@ -775,7 +775,14 @@ struct LpGrad {
 
 // Rows of at most 1024 logits: a group of L lanes each, in 16-byte vectors where
 // the row of x and the row of dx start at the same offset from a boundary.
-// (65536 x 258: 30.0 us by 8 lanes, 38.7 by 32; x 1000: 90 and 80.)
+// 8 lanes have 32 vectors under way, 32 lanes 128 but four times as many CTAs and
+// rows' coefficients: us by 8 / by 32 lanes,
+//
+//    rows      64          200         258         300         400         500
+//    9500   5.1/ 5.2    5.2/ 5.1    6.7/ 5.7    6.2/ 5.3    7.8/ 6.7
+//   15000   5.1/ 6.1    5.2/ 7.1    9.3/ 8.8    9.7/10.0   12.2/11.8
+//   19000   5.1/ 7.2    7.3/ 9.6   11.0/12.9   11.0/12.8   13.6/14.3
+//   65536   9.5/25.8   20.2/31.4   26.9/36.2   29.0/36.7   35.9/40.5   45.2/44.0 logits
 // A row without an upstream gradient is read no further than its lanes' first 16
 // values, which are fetched before that is known: 65536 x 1000, 90% ignored, 64.8
 // us (49.4 if it were known first, but 81.8 instead of 79.9 with none ignored).
@@ -894,8 +901,9 @@ __global__ void __launch_bounds__(LP_BWD_NT, 2048 / LP_BWD_NT) k_logprobs_bwd(co
 
 // Rows up to this long are held in registers.
 constexpr int64_t LP_SHORT = 1024;
-// Rows up to this long are 8 lanes' in the gradient, if there are many.
-constexpr int64_t LP_BWD_8 = 300;
+// Rows up to this long are 8 lanes' in the gradient (in two rounds of loads), and
+// up to this long if there are many (k_logprobs_bwd_short).
+constexpr int64_t LP_BWD_8 = 253, LP_BWD_8_MANY = 400;
 
 template <int L, bool TOP>
 static void launch_logprobs_short(const float* x, int64_t ld, const void* ids, int kind, int64_t R, int V, int K,
@@ -1008,7 +1016,7 @@ void launch_logprobs_bwd(const float* x, int64_t ld, const void* ids, int kind, 
 #define TP_LP_BWD(L)                                                                                                 \
   TP_LAUNCH(k_logprobs_bwd_short<L>, (unsigned)((R + 128 / L - 1) / (128 / L)), 128, 0, x, ld, ids, kind, stats, entropy, \
             dlogp, dentropy, R, (int)V, dx, ldd)
-    if (V <= LP_BWD_8 && R >= (int64_t)sm_count() * 64) TP_LP_BWD(8);
+    if (V <= LP_BWD_8 || (V <= LP_BWD_8_MANY && R >= (int64_t)sm_count() * 112)) TP_LP_BWD(8);
     else TP_LP_BWD(32);
 #undef TP_LP_BWD
     return;
