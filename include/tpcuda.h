@@ -434,7 +434,8 @@ TP_API int tp_clip_grad_norm_multi(const int64_t* grads, int n, float norm_type,
 /* New: the 2-norm of the group's gradients and the AdamW (kind 0) or Adam (1)
  * step that reads each gradient times coef: the same parameters and moments,
  * bit for bit, as tp_clip_grad_norm_multi followed by the step, with the
- * gradients left as they were. */
+ * gradients left as they were.  A tensor named twice, in one list or in two, is
+ * refused. */
 TP_API int tp_adam_clip_step_multi(int kind, const int64_t* params, const int64_t* grads, const int64_t* exp_avgs,
                                    const int64_t* exp_avg_sqs, int n, float lr, float beta1, float beta2, float eps,
                                    float weight_decay, float step_size, float inv_sqrt_bc2, float max_norm,

@@ -456,6 +456,19 @@ struct Group {
 static std::unordered_map<int64_t, Group> g_groups;
 static int64_t g_next_group = 1;
 
+using Span = std::pair<uintptr_t, uintptr_t>;  // of memory
+
+static void add_span(std::vector<Span>& spans, const float* p, int64_t n) {
+  if (n > 0) spans.emplace_back((uintptr_t)p, (uintptr_t)(p + n));
+}
+
+static bool disjoint(std::vector<Span> spans) {
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) return false;
+  return true;
+}
+
 // with_norm: with the partials and the overlap check of the gradient norm
 static Group build_group(const std::vector<OptRow>& rows, bool with_norm = false) {
   std::vector<OptChunk> chunks;
@@ -484,12 +497,9 @@ static Group build_group(const std::vector<OptRow>& rows, bool with_norm = false
   if (rb) TP_CUDA(cudaMemcpyAsync(g.rows, rows.data(), rb, cudaMemcpyHostToDevice, stream()));
   if (cb) TP_CUDA(cudaMemcpyAsync(g.chunks, chunks.data(), cb, cudaMemcpyHostToDevice, stream()));
   if (!with_norm) return g;
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  for (const OptRow& x : rows)
-    if (x.n > 0) spans.emplace_back((uintptr_t)x.g, (uintptr_t)(x.g + x.n));
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    if (spans[i].first < spans[i - 1].second) g.grads_disjoint = false;
+  std::vector<Span> spans;
+  for (const OptRow& x : rows) add_span(spans, x.g, x.n);
+  g.grads_disjoint = disjoint(std::move(spans));
   return g;
 }
 
@@ -765,6 +775,10 @@ TP_API int tp_adam_clip_step_multi(int kind, const int64_t* p, const int64_t* g,
       TP_REQUIRE(get(p[i]).phys == PHYS_F32 && get(g[i]).phys == PHYS_F32 && get(m[i]).phys == PHYS_F32 &&
                      get(v[i]).phys == PHYS_F32,
                  "%s: index tensors are not supported", what);
+    std::vector<Span> spans;
+    for (const OptRow& x : rows)
+      for (const float* q : {(const float*)x.p, x.g, (const float*)x.s0, (const float*)x.s1}) add_span(spans, q, x.n);
+    TP_REQUIRE(disjoint(std::move(spans)), "%s: a tensor is listed twice", what);
     TempGroup t(rows);
     Outputs o;
     const int64_t two[1] = {2};
