@@ -501,7 +501,10 @@ TP_API int tpk_token_embedding_backward(const float* dout, int64_t ldo, const vo
 
 /* ---- pointer-level optimizer kernels ---------------------------------------- */
 /* A tensor group is a device-side table of n (param, grad, state0, state1,
- * numel) rows built once; steps then take only hyper-parameters. */
+ * numel) rows built once; steps then take only hyper-parameters.  It is created
+ * outside of graph captures, where the entries above that take a list of tensors
+ * (tp_*_step, tp_*_step_multi, tp_clip_grad_norm_multi) are refused too: the list is uploaded
+ * from memory of the call. */
 TP_API int tpk_group_create(int n, float* const* params, float* const* grads, float* const* state0,
                             float* const* state1, const int64_t* numels, int64_t* out_group);
 /* The same with lo (NULL, or n pointers, each NULL or 16-byte aligned): the

@@ -471,6 +471,11 @@ static bool disjoint(std::vector<Span> spans) {
 
 // with_norm: with the partials and the overlap check of the gradient norm
 static Group build_group(const std::vector<OptRow>& rows, bool with_norm = false) {
+  // a replayed copy would read `rows` and `chunks` after they are gone
+  cudaStreamCaptureStatus capture;
+  TP_CUDA(cudaStreamIsCapturing(stream(), &capture));
+  TP_REQUIRE(capture == cudaStreamCaptureStatusNone,
+             "a list of tensors cannot be uploaded in a graph capture: create a tensor group before it");
   std::vector<OptChunk> chunks;
   for (size_t r = 0; r < rows.size(); ++r) {
     const OptRow& x = rows[r];
