@@ -33,3 +33,11 @@ def test_the_most_positions_of_an_embedding_gradient(lib):
     b = ctypes.c_int64(-1)
     assert lib.tpk_token_embedding_backward_ws(MOST, 1, 1, ctypes.byref(b)) == 0
     assert b.value > 4 * 4 * MOST  # positions and tokens, split and sorted
+
+
+def test_norm_buffers_off_a_value_boundary(lib):
+    for off in (1, 2, 3):
+        for status in (lib.tpk_group_grad_norm(987654321, 2.0, 1.0, P + off),
+                       lib.tpk_group_clip_grad_norm(987654321, 2.0, 1.0, P + off),
+                       lib.tpk_adam_group_scaled(987654321, 0, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1e-3, 1.0, P + off)):
+            assert status == ARG and b"aligned" in lib.tp_last_error()

@@ -719,6 +719,7 @@ TP_API int tpk_group_grad_norm(int64_t group, float norm_type, float max_norm, f
     const char* what = "group_grad_norm";
     const int p = norm_code(norm_type, max_norm, what);
     TP_REQUIRE(norm_coef, "%s: norm_coef is NULL", what);
+    check_aligned({norm_coef}, what);
     auto it = g_groups.find(group);
     TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
     launch_grad_norm(it->second, p, max_norm, false, norm_coef, what);
@@ -730,6 +731,7 @@ TP_API int tpk_group_clip_grad_norm(int64_t group, float norm_type, float max_no
     const char* what = "group_clip_grad_norm";
     const int p = norm_code(norm_type, max_norm, what);
     TP_REQUIRE(norm_coef, "%s: norm_coef is NULL", what);
+    check_aligned({norm_coef}, what);
     auto it = g_groups.find(group);
     TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
     launch_grad_norm(it->second, p, max_norm, true, norm_coef, what);
@@ -741,6 +743,7 @@ TP_API int tpk_adam_group_scaled(int64_t group, int kind, float lr, float b1, fl
   return guard([&] {
     TP_REQUIRE(kind == 0 || kind == 1, "adam_group_scaled: kind must be 0 (AdamW) or 1 (Adam), got %d", kind);
     TP_REQUIRE(grad_scale, "adam_group_scaled: grad_scale is NULL");
+    check_aligned({grad_scale}, "adam_group_scaled");
     auto it = g_groups.find(group);
     TP_REQUIRE(it != g_groups.end(), "unknown tensor group %lld", (long long)group);
     launch_adam_group(it->second, kind == 0, adam_hp(lr, b1, b2, eps, wd, ss, isb), grad_scale);
