@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(256) k_embed_few(const float* __restrict__ dou
 // are n D 4 bytes from HBM.)
 constexpr int SORT_NT = 1024;
 constexpr int SORT_WARPS = SORT_NT / 32;
-constexpr int LEAST_G = 7, MOST_G = 10;   // log2 of the CTAs: 128 for 148 SMs, or more
+constexpr int EMB_SMS = 148;              // of a B200: a workspace's size is asked for without a device too
+constexpr int LEAST_G = 7, MOST_G = 10;   // log2 of the CTAs: 128 for its SMs, or more
 constexpr int SORT_TOKENS = 1024;         // tokens of one CTA, at most (a thread each in the scan)
 constexpr int SORT_WORDS = 1024;          // positions / 32 of one launch: their hits are kept in shared memory
 constexpr int64_t SORT_READS = (int64_t)1 << 22;  // ids that the CTAs of one launch read in all, at most
@@ -568,8 +569,9 @@ __device__ __forceinline__ void embed_zero(const EmbedSort& e, const EmbedSum& a
     clear_row(a.dtable + (v0 + __ffs(some) - 1) * a.ld, D, lane, 32);
 }
 
-// (4 CTAs to an SM with the old values in flight: its registers would leave 3, and
-// 131622 x 332 added then takes 94.5 us instead of 87.4; 8 would spill.)
+// (4 CTAs to an SM with the old values in flight, at 128 registers and 24 bytes
+// spilled: its registers would leave 3, and 131622 x 332 added then takes 94.5 us
+// instead of 87.4; 8 CTAs would spill 920.)
 template <int VEC, bool ACC>
 __global__ void __launch_bounds__(EMB_NT, VEC == 4 && ACC ? 4 : 1) k_embed_sum(const EmbedSort e, const EmbedSum a) {
   ::tp::pdl_enter();
@@ -773,7 +775,7 @@ struct EmbedPlan {
     while (g < MOST_G && ((int64_t)SORT_TOKENS << g) < V) ++g;
     per = (V + (1 << g) - 1) >> g;
     const int64_t work = n / 64 * D / 512;  // CTAs of 512 columns by 64 positions
-    T = work >= 148 * 4 ? 64 : (work >= 148 * 2 ? 32 : 16);
+    T = work >= EMB_SMS * 4 ? 64 : (work >= EMB_SMS * 2 ? 32 : 16);
     tiles = (n + T - 1) / T;
     ldp = (D + 3) / 4 * 4;
     auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
@@ -785,7 +787,7 @@ struct EmbedPlan {
     // launch, 27.5 split first; 65536 ids 33.9 and 31.6
     split = per > SORT_TOKENS || n << g > SORT_READS;
     const int64_t words = (n + 31) / 32;
-    share = (words + 147) / 148;
+    share = (words + EMB_SMS - 1) / EMB_SMS;
     B = split ? (int)((words + share - 1) / share) : 0;
     count = cut + up(tiles * 8);
     first = count + up((int64_t)B * 4 << g);

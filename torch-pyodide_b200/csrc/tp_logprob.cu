@@ -14,7 +14,7 @@
 // What bounds it: the logits' bytes.  Per logit there are about 7 issue slots (a
 // difference, a clamp, a product, an exponential, two sums, a maximum), one of
 // them a MUFU, of the 21 slots and 2.8 MUFU that an SM has in the time HBM takes
-// to bring it.  8192 x 131072: 591 us, 7.3 TB/s read.
+// to bring it.  8192 x 131072: 588 us, 7.3 TB/s read.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(128) k_logprobs_short(const float* __restrict_
 // row as well as many and no workspace is shared between calls.  (One row of
 // 32000 with 20 alternatives: 7.0 us in eight parts, 36 us by a warp.  2000 rows of
 // 50021 in two parts each: 95 us against 73, the exchange costs more than it
-// balances.)  1999 x 50021 with 5 alternatives: 70 us, 5.7 TB/s: the last, uneven
+// balances.)  1999 x 50021 with 5 alternatives: 71 us, 5.6 TB/s: the last, uneven
 // wave of rows is most of what is missing.
 //
 // The alternatives cost the walk little: of the q-th vectors of all its batches (a
